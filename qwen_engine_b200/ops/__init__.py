@@ -1674,6 +1674,127 @@ def copy_pages(cache: torch.Tensor, pairs: torch.Tensor) -> None:
                                _stream()), "copy_pages")
 
 
+def _here(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Launches go to the current device's stream: the operands must live there."""
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != _current_device():
+            raise KernelRefused(f"{name}: a tensor on {t.device} while the current device is cuda:{_current_device()}")
+
+
+def _same_or_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one shape are the same memory, or share none of it."""
+    pa, pb, n = a.data_ptr(), b.data_ptr(), a.numel() * a.element_size()
+    return pa == pb or pa + n <= pb or pb + n <= pa
+
+
+ATTENTION_WEIGHTS_MAX_PARTS = 64      # parts of a row's keys at most, where the rows alone do not fill the SMs
+
+
+def _attention_weights_parts(row_tiles: int, heads: int, requests: int, max_total: int) -> int:
+    """In how many parts the rows' keys are cut: two CTAs an SM, and 256 keys a part at least."""
+    return max(1, min(-(-FLASH_TARGET_CTAS // max(1, row_tiles * heads * requests)), -(-max_total // 256), ATTENTION_WEIGHTS_MAX_PARTS))
+
+
+def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables: torch.Tensor, ctx, weights: torch.Tensor,
+                         out: torch.Tensor, scale: float, window: int, num_heads: int, num_kv_heads: int, head_dim: int, alloc,
+                         positions: Optional[torch.Tensor] = None, counted: Optional[torch.Tensor] = None,
+                         slopes: Optional[torch.Tensor] = None, softcap: float = 0.0, sinks: Optional[torch.Tensor] = None) -> None:
+    """What every cached key has received of the softmax's weights: for request r in slot s = ctx.slot_ids[r] and kv head c,
+    out[s, c, j] = weights[s, c, j] (0 for the step's own tokens, j >= ctx_lens[r]) + the sum over the request's rows and over
+    the query heads of the kv head's group of the weight that the row puts on key j, for every j below ctx_lens[r] + its tokens;
+    what lies behind stays as it is.  The step's keys are in the cache already (``paged_attention`` reads the same).
+
+    weights and out: float32 [slots, Hkv, capacity], the same tensor or two that share no memory; two requests never have
+    one slot.  qkv [T, >= Hq D] in the cache's type (float32 or bfloat16; rows may be strided), kv_pages [pages, planes, Hkv, page, D], plane 0 the keys.
+    ``positions`` (int32, weights' shape): positions[s, c, ctx_lens[r] + i] gets ctx.positions of the request's i-th token.
+    ``counted`` (int32 [R]): only so many of a request's first rows count (what ``verify_drafts`` leaves in its counts);
+    the others' keys get no weight.
+    ``window``, ``slopes``, ``softcap``, ``sinks``: as in ``paged_attention``.  Keys that lie in no page get no weight; distances
+    are of places in the cache, so that a window or a distance bias goes with a cache that nothing was evicted from.
+    ``alloc(shape, dtype)`` gives scratch memory.  Float32 sums in one order: equal calls give equal bits."""
+    Hq, Hkv, D = num_heads, num_kv_heads, head_dim
+    T, R, planes = qkv.shape[0], int(ctx.num_reqs), int(kv_pages.shape[1]) if kv_pages.dim() == 5 else 0
+    _rows(qkv, "accumulate_attention: qkv")
+    _need(Hkv >= 1 and Hq % Hkv == 0 and D >= 1, "accumulate_attention: the query heads must be a multiple of the kv heads")
+    _need(qkv.shape[1] >= Hq * D, "accumulate_attention: qkv must hold Hq D columns of queries")
+    _need(kv_pages.dtype == qkv.dtype and kv_pages.dim() == 5 and kv_pages.is_contiguous() and planes >= 1
+          and kv_pages.shape[2] == Hkv and kv_pages.shape[4] == D,
+          "accumulate_attention: kv_pages must be [pages, planes, Hkv, page, D] in q's dtype")
+    _i32(block_tables, "block_tables")
+    _need(block_tables.dim() == 2 and block_tables.shape[0] == R, "accumulate_attention: block_tables must be [R, blocks]")
+    _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[1] == Hkv and weights.is_contiguous()
+          and out.dtype == torch.float32 and out.shape == weights.shape and out.is_contiguous(),
+          "accumulate_attention: weights and out must be contiguous float32 [slots, Hkv, capacity]")
+    _need(_same_or_apart(weights, out), "accumulate_attention: weights and out must be one tensor or share no memory")
+    _need(positions is None or (positions.dtype == torch.int32 and positions.shape == weights.shape and positions.is_contiguous()),
+          "accumulate_attention: positions must be int32 [slots, Hkv, capacity]")
+    _need(counted is None or (counted.dtype == torch.int32 and counted.shape == (R,) and counted.is_contiguous()),
+          "accumulate_attention: counted must be int32 [R]")
+    for t, name in ((slopes, "slopes"), (sinks, "sinks")):
+        _need(t is None or (t.dtype == torch.float32 and t.numel() == Hq and t.is_contiguous()), f"accumulate_attention: {name} must be float32 [Hq]")
+    _need(scale > 0.0 and softcap >= 0.0, "accumulate_attention: the scale must be positive, the cap not negative")
+    page = int(kv_pages.shape[3])
+    longest = max((q + c for q, c in zip(ctx.q_lens_host, ctx.ctx_lens_host)), default=0)
+    _need(longest <= weights.shape[2], f"accumulate_attention: a request of {longest} tokens in {weights.shape[2]} places")
+    _need(longest <= int(block_tables.shape[1]) * page, f"accumulate_attention: a request of {longest} tokens in {int(block_tables.shape[1])} blocks of {page}")
+    _here("accumulate_attention", qkv, kv_pages, block_tables, weights, out, positions, counted, slopes, sinks, ctx.cu_q)
+    if R == 0 or T == 0:
+        return
+    max_q, max_total = max(ctx.q_lens_host), min(int(weights.shape[2]), int(block_tables.shape[1]) * page)
+    parts = _attention_weights_parts(-(-max_q * (Hq // Hkv) // 64), Hkv, R, max_total)
+    stats = alloc((T * Hq, parts, 2), torch.float32)
+    _check(lib().qe_attention_weights(
+        _ptr(qkv), ctypes.c_long(qkv.stride(0)), T, _ptr(kv_pages), int(kv_pages.shape[0]), planes, _ptr(block_tables),
+        int(block_tables.shape[1]), _ptr(ctx.cu_q), _ptr(ctx.ctx_lens), _ptr(ctx.slot_ids), _ptr(counted), _ptr(ctx.positions),
+        _ptr(positions), _ptr(weights), _ptr(out), int(weights.shape[0]), ctypes.c_long(weights.shape[2]), R, Hq, Hkv, D, page,
+        int(window), ctypes.c_float(scale), ctypes.c_float(softcap), _ptr(slopes), _ptr(sinks), _ptr(stats), parts, max_q, max_total,
+        _dt(qkv), _stream()), "accumulate_attention")
+
+
+def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,
+                 positions: torch.Tensor, weights_out: torch.Tensor, positions_out: torch.Tensor, keep: int, first: int, recent: int,
+                 alloc) -> None:
+    """Bring requests' caches down to ``keep`` entries, for every layer and kv head by itself: request r holds lens[r] entries
+    (places 0 .. lens[r] - 1 of its block table) and min(lens[r], keep) afterwards.  Entries at positions below ``first`` and
+    less than ``recent`` behind the request's latest position stay; of the others those with the largest weights, the lowest
+    place among equals (NaN counts as the lowest).  Entries that stay and lie behind place ``keep`` move, in their order,
+    into the places before it that come free, in theirs; the others do not move, so the order of a cache's keys is not kept
+    (attention without a window or a distance bias does not look at it; ``positions`` say which token is where).
+
+    cache: a group's tensor [layers, pages, planes, Hkv, page, D], all planes of an entry move; block_tables int32 [R, blocks];
+    slot_ids int32 [R]: the rows of ``weights`` (float32) and ``positions`` (int32), both [layers, slots, Hkv, capacity], that
+    belong to the requests; lens int32 [R] on the device.  weights_out and positions_out get the kept entries' weights and
+    positions in their new places (places from min(lens, keep) on stay as they are); they may be the inputs themselves.
+    A request's positions are distinct, pages it moves within are its own (not shared with another request), no two requests
+    have one slot.  ``alloc(shape, dtype)`` gives scratch memory."""
+    _need(cache.dim() == 6 and cache.is_contiguous(), "evict_tokens: cache must be contiguous [layers, pages, planes, Hkv, page, D]")
+    S, pages, planes, Hkv, page, D = (int(n) for n in cache.shape)
+    _i32(block_tables, "block_tables")
+    _i32(slot_ids, "slot_ids")
+    _i32(lens, "lens")
+    R = lens.numel()
+    _need(block_tables.dim() == 2 and block_tables.shape[0] == R and slot_ids.numel() == R, "evict_tokens: a block table, a slot and a length for every request")
+    _need(weights.dtype == torch.float32 and weights.dim() == 4 and weights.shape[0] == S and weights.shape[2] == Hkv and weights.is_contiguous(),
+          "evict_tokens: weights must be contiguous float32 [layers, slots, Hkv, capacity]")
+    _need(positions.dtype == torch.int32 and positions.shape == weights.shape and positions.is_contiguous(),
+          "evict_tokens: positions must be contiguous int32 [layers, slots, Hkv, capacity]")
+    for t, like, name in ((weights_out, weights, "weights_out"), (positions_out, positions, "positions_out")):
+        _need(t.dtype == like.dtype and t.shape == like.shape and t.is_contiguous(), f"evict_tokens: {name} must be like its input")
+        _need(_same_or_apart(t, like), f"evict_tokens: {name} must be its input or share no memory with it")
+    _need(int(keep) >= 1 and int(first) >= 0 and int(recent) >= 0, "evict_tokens: keep must be at least 1, first and recent not negative")
+    _need(int(first) + int(recent) <= int(keep), f"evict_tokens: {first} first and {recent} recent entries do not fit a budget of {keep}")
+    _here("evict_tokens", cache, block_tables, slot_ids, lens, weights, positions, weights_out, positions_out)
+    if R == 0 or S == 0:
+        return
+    capacity = min(int(weights.shape[3]), int(block_tables.shape[1]) * page)
+    keep = min(int(keep), max(capacity, 1))
+    moves = alloc((S, R, Hkv, 1 + 2 * keep), torch.int32)
+    _check(lib().qe_evict_tokens(
+        _ptr(cache), S, pages, planes, Hkv, page, D * cache.element_size(), _ptr(block_tables), int(block_tables.shape[1]), _ptr(slot_ids),
+        _ptr(lens), R, _ptr(weights), _ptr(positions), _ptr(weights_out), _ptr(positions_out), int(weights.shape[1]),
+        ctypes.c_long(weights.shape[3]), capacity, keep, int(first), int(recent), _ptr(moves), _stream()), "evict_tokens")
+
+
 def silu_mul(gate_up: torch.Tensor, out: torch.Tensor) -> None:
     """out[t, i] = silu(gate_up[t, i]) * gate_up[t, I + i]."""
     T, I2 = gate_up.shape
@@ -2390,3 +2511,46 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     _i32(top_k, "top_k")
     _i32(out, "out")
     _check(lib().qe_sample(_ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(uniform), _ptr(out), N, V, _stream()), "sample")
+
+
+VERIFY_CHUNKS = 8     # chunks of a row of logits, each with its own maximum and sum (the CTAs of a cluster)
+
+
+def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, draft_logits: Optional[torch.Tensor], row_starts: torch.Tensor,
+                  temperature: torch.Tensor, top_k: torch.Tensor, uniform: torch.Tensor, tokens: torch.Tensor, counts: torch.Tensor,
+                  alloc) -> None:
+    """Hold drafted tokens against the target's probabilities.  Request r has the rows row_starts[r] .. row_starts[r + 1] - 1
+    of ``logits`` (float32 [N, V]), one more than it has drafts: row i is the target's for the place of draft i, the last row
+    for the token behind all drafts.  ``draft_tokens`` int32 [N - R] are the requests' drafts one behind the other, and
+    ``draft_logits`` float32 [N - R, V] what they were drawn from (``sample`` with the request's temperature and top_k), or None
+    where they were not drawn but found (then a draft's own probability is 1).
+
+    With p and q the distributions that ``sample`` would draw from (temperature 0: all on the argmax), draft i stands if the drafts
+    before it do and uniform[row] q(draft) < p(draft).  The token behind the a drafts that stand is drawn with the uniform number
+    of the request's LAST row: from max(p - q, 0) where draft a fell (from p, where that is all zero), from p of the last row where all
+    stand; the first index whose running sum exceeds uniform times the whole.  Drawn so, the tokens are distributed as the target's.
+
+    temperature float32 [R], top_k int32 [R] (0: the whole vocabulary; ties at the threshold are all kept), uniform float32 [N] in [0, 1).
+    tokens int32 [N]: the request's rows get the drafts that stand, the drawn token, and -1 behind it; counts int32 [R]: how many
+    tokens that are, a + 1 (so many of the request's rows are now part of its text).  A draft outside the vocabulary falls; NaN
+    counts as -inf; a row without any logit above -inf lets no draft stand and gives token 0.  ``alloc(shape, dtype)`` gives scratch memory."""
+    N, V = logits.shape
+    R = counts.numel()
+    _need(logits.dtype == torch.float32 and logits.is_contiguous(), "verify_drafts: logits must be contiguous float32 [N, V]")
+    for t, n, name in ((draft_tokens, N - R, "draft_tokens"), (row_starts, R + 1, "row_starts"), (top_k, R, "top_k"), (tokens, N, "tokens"),
+                       (counts, R, "counts")):
+        _i32(t, f"verify_drafts: {name}")
+        _need(t.numel() == n, f"verify_drafts: {name} has {t.numel()} entries, not {n}")
+    for t, n, name in ((temperature, R, "temperature"), (uniform, N, "uniform")):
+        _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, f"verify_drafts: {name} must be float32 with {n} entries")
+    _need(draft_logits is None or (draft_logits.dtype == torch.float32 and draft_logits.is_contiguous() and draft_logits.shape == (N - R, V)),
+          "verify_drafts: draft_logits must be contiguous float32 [N - R, V]")
+    _here("verify_drafts", logits, draft_tokens, draft_logits, row_starts, temperature, top_k, uniform, tokens, counts)
+    if R == 0:
+        return
+    rows = N + (N - R if draft_logits is not None else 0)
+    parts = alloc((rows, VERIFY_CHUNKS, 2), torch.float64)        # 16 bytes a chunk: sum, maximum, its place
+    thresholds = alloc((rows,), torch.int32)
+    _check(lib().qe_verify_drafts(_ptr(logits), _ptr(draft_tokens), _ptr(draft_logits if N > R else None), _ptr(row_starts), _ptr(temperature),
+                                  _ptr(top_k), _ptr(uniform), _ptr(tokens), _ptr(counts), _ptr(parts), _ptr(thresholds), N, R, V, _stream()),
+           "verify_drafts")

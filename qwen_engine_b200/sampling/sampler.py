@@ -5,7 +5,7 @@ request's tokens do not depend on which other requests share its steps, and a
 plain implementation on the CPU can reproduce them."""
 from __future__ import annotations
 
-from typing import Sequence
+from typing import Optional, Sequence
 
 import torch
 
@@ -52,6 +52,26 @@ class SampledTokens:
         return self._host.tolist()
 
 
+class VerifiedTokens:
+    """The tokens of one verification: on the device at once (``counts`` int32 [R], how many tokens each request gained,
+    and ``tokens`` int32 [N] in the rows' layout, -1 behind them), on the host when ``read()`` is called."""
+
+    def __init__(self, counts: torch.Tensor, tokens: torch.Tensor, lengths: Sequence[int]):
+        self.counts, self.tokens = counts, tokens
+        self._lengths = list(lengths)
+        self._both = SampledTokens(torch.cat([counts, tokens]))
+
+    def read(self) -> list[list[int]]:
+        """A list of tokens per request: its drafts that stand, and the one behind them."""
+        both = self._both.read()
+        R = len(self._lengths)
+        out, at = [], R
+        for n, count in zip(self._lengths, both[:R]):
+            out.append(both[at:at + count])
+            at += n
+        return out
+
+
 class Sampler:
     def __init__(self, device):
         self.device = torch.device(device)
@@ -77,3 +97,32 @@ class Sampler:
                 topk = topk.pin_memory().to(self.device, non_blocking=True)
             ops.sample(logits, meta[0].contiguous(), topk, meta[1].contiguous(), out)
         return SampledTokens(out)
+
+    def verify(self, logits: torch.Tensor, params: Sequence[SamplingParams], drafts: Sequence[Sequence[int]],
+               uniforms: Sequence[Sequence[float]], draft_logits: Optional[torch.Tensor] = None) -> list[list[int]]:
+        """The tokens each request gains from a step that ran its newest token and its drafts: see ``verify_async``."""
+        return self.verify_async(logits, params, drafts, uniforms, draft_logits).read()
+
+    def verify_async(self, logits: torch.Tensor, params: Sequence[SamplingParams], drafts: Sequence[Sequence[int]],
+                     uniforms: Sequence[Sequence[float]], draft_logits: Optional[torch.Tensor] = None) -> VerifiedTokens:
+        """Hold drafted tokens against the target's logits without waiting for the device.  ``logits`` float32 [N, V]: for
+        request r one row more than it has ``drafts``, in the order of the step's wanted places; ``uniforms[r]`` has a number
+        for each of its rows (the last one draws the token behind the drafts that stand).  ``draft_logits`` float32 [N - R, V]:
+        what the drafts were drawn from, or None for drafts that were found."""
+        R = len(params)
+        lengths = [len(d) + 1 for d in drafts]
+        if len(drafts) != R or [len(u) for u in uniforms] != lengths or logits.shape[0] != sum(lengths):
+            raise ValueError("verify: one list of drafts per request, one uniform number and one row of logits per draft and one more")
+        starts = [0]
+        for n in lengths:
+            starts.append(starts[-1] + n)
+        ints = torch.tensor(starts + [p.top_k for p in params] + [int(t) for d in drafts for t in d], dtype=torch.int32)
+        floats = torch.tensor([p.temperature for p in params] + [float(u) for us in uniforms for u in us], dtype=torch.float32)
+        if self.device.type == "cuda":
+            ints = ints.pin_memory().to(self.device, non_blocking=True)
+            floats = floats.pin_memory().to(self.device, non_blocking=True)
+        tokens = torch.empty(starts[-1], dtype=torch.int32, device=self.device)
+        counts = torch.empty(R, dtype=torch.int32, device=self.device)
+        ops.verify_drafts(logits, ints[2 * R + 1:], draft_logits, ints[:R + 1], floats[:R], ints[R + 1:2 * R + 1], floats[R:], tokens, counts,
+                          lambda shape, dtype: torch.empty(shape, dtype=dtype, device=self.device))
+        return VerifiedTokens(counts, tokens, lengths)

@@ -1,0 +1,559 @@
+"""Verification of drafted tokens, gathered attention weights and eviction against their definitions in 64 bits
+(tests/plain_drafts.py): types, head layouts, lengths from none and one to long ones, odd sizes, strides, masks, ties."""
+import math
+import random
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import plain_drafts
+from qwen_engine_b200 import ops
+from qwen_engine_b200.sampling import Sampler, SamplingParams
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _alloc(shape, dtype):
+    return torch.empty(shape, dtype=dtype, device=DEV)
+
+
+# ---- verification ----------------------------------------------------------------------------------------------------------
+
+def _verify_case(R, drafts, V, seed, model=True, top_ks=(0,), temps=(0.8,), scale=2.0):
+    g = torch.Generator().manual_seed(seed)
+    rnd = random.Random(seed)
+    ns = [rnd.choice(drafts) for _ in range(R)]
+    starts = [0]
+    for n in ns:
+        starts.append(starts[-1] + n + 1)
+    N = starts[-1]
+    logits = torch.randn(N, V, generator=g) * scale
+    rows = [starts[r] + i for r in range(R) for i in range(ns[r])]
+    draft_logits = logits[rows] + 0.5 * torch.randn(len(rows), V, generator=g) if model else None
+    tokens = (draft_logits if model else logits[rows]).add(2 * torch.randn(len(rows), V, generator=g)).argmax(1).to(torch.int32)
+    return dict(logits=logits, draft_tokens=tokens, draft_logits=draft_logits, row_starts=torch.tensor(starts, dtype=torch.int32),
+                temperature=torch.tensor([rnd.choice(temps) for _ in range(R)]), top_k=torch.tensor([rnd.choice(top_ks) for _ in range(R)], dtype=torch.int32),
+                uniform=torch.rand(N, generator=g))
+
+
+def _verify(c, **other):
+    d = {k: (v.to(DEV) if isinstance(v, torch.Tensor) else v) for k, v in {**c, **other}.items()}
+    N, R = d["logits"].shape[0], d["temperature"].numel()
+    tokens = torch.full((N,), -7, dtype=torch.int32, device=DEV)
+    counts = torch.full((R,), -7, dtype=torch.int32, device=DEV)
+    ops.verify_drafts(d["logits"], d["draft_tokens"], d["draft_logits"], d["row_starts"], d["temperature"], d["top_k"], d["uniform"],
+                      tokens, counts, _alloc)
+    return tokens.cpu(), counts.cpu()
+
+
+def _same(got, want):
+    assert torch.equal(got[1], want[1]), (got[1].tolist(), want[1].tolist())
+    assert torch.equal(got[0], want[0]), [(i, a, b) for i, (a, b) in enumerate(zip(got[0].tolist(), want[0].tolist())) if a != b][:5]
+
+
+@pytest.mark.parametrize("model", [True, False])
+@pytest.mark.parametrize("R,drafts,V", [(1, [4], 151936), (7, [0, 1, 2, 5], 1001), (33, [3], 130), (3, [0], 389), (2, [40, 1], 77), (5, [2], 1), (9, [1, 3], 2),
+                                        (4, [2, 6], 32003)])
+def test_verify_drafts(model, R, drafts, V):
+    for seed in range(3):
+        c = _verify_case(R, drafts, V, 10 * seed + R, model)
+        _same(_verify(c), plain_drafts.verify(**c))
+
+
+@pytest.mark.parametrize("model", [True, False])
+@pytest.mark.parametrize("V", [97, 4099, 70001])
+def test_verify_drafts_with_top_k_and_greedy_requests(model, V):
+    for seed in range(3):
+        c = _verify_case(12, [0, 1, 4], V, 77 + seed, model, top_ks=(0, 1, 2, 50, 1000, V, V + 3), temps=(0.0, 0.3, 1.0, 2.5))
+        _same(_verify(c), plain_drafts.verify(**c))
+
+
+def test_verify_drafts_with_ties_at_the_threshold_and_coarse_logits():
+    """Logits in steps of a half: many equal the top_k-th largest (all are kept) and many the largest (the lowest place is the argmax)."""
+    for seed in range(3):
+        c = _verify_case(8, [3], 515, 200 + seed, True, top_ks=(1, 5, 40), temps=(0.0, 0.7))
+        c["logits"], c["draft_logits"] = (c["logits"] * 2).round() / 2, (c["draft_logits"] * 2).round() / 2
+        c["logits"][:, ::7] *= -0.0
+        _same(_verify(c), plain_drafts.verify(**c))
+
+
+def test_verify_drafts_with_masked_logits():
+    """-inf, NaN and the type's lowest value in masked places, rows without any finite logit, +inf, drafts that are masked or outside the vocabulary."""
+    low = torch.finfo(torch.float32).min
+    for seed in range(4):
+        for model in (True, False):
+            c = _verify_case(10, [2, 4], 333, 300 + seed, model, top_ks=(0, 3, 30), temps=(0.0, 0.6, 1.0))
+            g = torch.Generator().manual_seed(seed)
+            N = c["logits"].shape[0]
+            for x in [c["logits"]] + ([c["draft_logits"]] if model else []):
+                m = torch.rand(x.shape, generator=g)
+                x[m < 0.3] = -math.inf
+                x[(m >= 0.3) & (m < 0.35)] = math.nan
+                x[(m >= 0.35) & (m < 0.5)] = low
+            c["logits"][1] = -math.inf
+            c["logits"][4] = math.nan
+            c["logits"][6] = low
+            c["logits"][8, 5] = c["logits"][8, 100] = math.inf
+            if model:
+                c["draft_logits"][2] = -math.inf
+            c["draft_tokens"][3], c["draft_tokens"][5] = 333, -1
+            _same(_verify(c), plain_drafts.verify(**c))
+
+
+def test_verify_drafts_at_the_ends_of_the_uniform_numbers():
+    c = _verify_case(6, [3], 501, 5, True)
+    for u in (0.0, 1.0 - 2.0 ** -24):
+        c["uniform"][:] = u
+        _same(_verify(c), plain_drafts.verify(**c))
+    # the draft's distribution is the target's: every draft stands, whatever the number
+    starts = c["row_starts"].tolist()
+    c["draft_logits"] = c["logits"][[starts[r] + i for r in range(6) for i in range(3)]].clone()
+    c["uniform"][:] = 1.0 - 2.0 ** -24
+    got = _verify(c)
+    assert got[1].tolist() == [4] * 6
+    _same(got, plain_drafts.verify(**c))
+
+
+def test_verify_drafts_off_a_16_byte_boundary():
+    c = _verify_case(4, [2], 1003, 6, True, top_ks=(0, 9))
+    want = plain_drafts.verify(**c)
+    for shift in (1, 2, 3):
+        def moved(x):
+            room = torch.zeros(x.numel() + 4, device=DEV)
+            v = room[shift:shift + x.numel()].view(x.shape)
+            v.copy_(x)
+            return v
+        _same(_verify(c, logits=moved(c["logits"]), draft_logits=moved(c["draft_logits"])), want)
+
+
+@pytest.mark.parametrize("model", [True, False])
+def test_verified_tokens_are_distributed_as_the_targets(model):
+    """Many requests with one target: the first token each gains (the draft, or the one in its place) has the target's
+    probabilities.  A count of n trials is off by 5 standard deviations, sqrt(n p (1 - p)), once in millions."""
+    R, V = 20000, 7
+    g = torch.Generator().manual_seed(3)
+    target, other = torch.randn(V, generator=g) * 1.5, torch.randn(V, generator=g) * 1.5
+    q = torch.softmax(other, 0)
+    drafts = torch.multinomial(q, R, replacement=True, generator=g).to(torch.int32) if model else torch.full((R,), 2, dtype=torch.int32)
+    c = dict(logits=target.expand(2 * R, V).contiguous(), draft_tokens=drafts, draft_logits=other.expand(R, V).contiguous() if model else None,
+             row_starts=torch.arange(0, 2 * R + 1, 2, dtype=torch.int32), temperature=torch.ones(R), top_k=torch.zeros(R, dtype=torch.int32),
+             uniform=torch.rand(2 * R, generator=g))
+    tokens, counts = _verify(c)
+    p = torch.softmax(target.double(), 0)
+    seen = torch.bincount(tokens[::2].long(), minlength=V).double()
+    assert (torch.abs(seen - R * p) <= 5 * torch.sqrt(R * p * (1 - p))).all(), (seen / R, p)
+    assert int(tokens[::2].min()) >= 0 and 0.1 < float((counts == 2).double().mean()) < 0.99
+
+
+def test_verify_drafts_of_a_request_without_rows():
+    """It gets no tokens, and the requests in front of it theirs."""
+    c = _verify_case(2, [2], 50, 9, True)
+    want = plain_drafts.verify(**c)
+    c["row_starts"] = torch.tensor([0, 3, 6, 6], dtype=torch.int32)
+    c["temperature"], c["top_k"] = torch.cat([c["temperature"], torch.ones(1)]), torch.cat([c["top_k"], torch.zeros(1, dtype=torch.int32)])
+    c["draft_tokens"], c["draft_logits"] = c["draft_tokens"][:3], c["draft_logits"][:3]      # (N - R of them)
+    tokens, counts = _verify(c)
+    assert counts[2] == 0 and counts[0] == want[1][0] and torch.equal(tokens[:3], want[0][:3])
+
+
+def test_the_sampler_verifies():
+    V = 301
+    c = _verify_case(4, [0, 2, 3], V, 12, True, top_ks=(0, 20), temps=(0.0, 0.9))
+    starts = c["row_starts"].tolist()
+    params = [SamplingParams(temperature=float(t), top_k=int(k)) for t, k in zip(c["temperature"], c["top_k"])]
+    drafts = [c["draft_tokens"][starts[r] - r:starts[r + 1] - r - 1].tolist() for r in range(4)]
+    uniforms = [c["uniform"][starts[r]:starts[r + 1]].tolist() for r in range(4)]
+    for model in (True, False):
+        dl = c["draft_logits"] if model else None
+        tokens, counts = plain_drafts.verify(**{**c, "draft_logits": dl})
+        got = Sampler(DEV).verify(c["logits"].to(DEV), params, drafts, uniforms, dl.to(DEV) if model else None)
+        assert got == [tokens[starts[r]:starts[r] + counts[r]].tolist() for r in range(4)]
+    # no drafts: what the sampler draws
+    rows = c["logits"][:4].contiguous().to(DEV)
+    got = Sampler(DEV).verify(rows, params, [[]] * 4, [[u] for u in (0.1, 0.4, 0.6, 0.9)])
+    assert [t[0] for t in got] == Sampler(DEV).sample(rows, params, [0.1, 0.4, 0.6, 0.9])
+
+
+# ---- gathered attention weights -------------------------------------------------------------------------------------------------
+
+def _weights_case(dtype, Hq, Hkv, D, P, q_lens, ctx_lens, seed, planes=2, counted=None, extra=3, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    R, T = len(q_lens), sum(q_lens)
+    totals = [a + b for a, b in zip(q_lens, ctx_lens)]
+    blocks = [-(-t // P) for t in totals]
+    pages = sum(blocks) + 2
+    order = iter(torch.randperm(pages, generator=g).tolist())
+    table = torch.full((R, max(blocks) + 1), -1, dtype=torch.int32)
+    for r, nb in enumerate(blocks):
+        for b in range(nb):
+            table[r, b] = next(order)
+    cap, slots = max(totals) + extra, R + 2
+    cu = [0]
+    for n in q_lens:
+        cu.append(cu[-1] + n)
+    return dict(qkv=(torch.randn(T, (Hq + 2 * Hkv) * D, generator=g) * std).to(dtype), pages=torch.randn(pages, planes, Hkv, P, D, generator=g).to(dtype),
+                table=table, cu=torch.tensor(cu, dtype=torch.int32), ctx=torch.tensor(ctx_lens, dtype=torch.int32),
+                slots=torch.randperm(slots, generator=g)[:R].to(torch.int32), weights=torch.rand(slots, Hkv, cap, generator=g),
+                step_positions=torch.randint(0, 10 ** 6, (T,), generator=g, dtype=torch.int32), q_lens=list(q_lens), ctx_lens=list(ctx_lens),
+                counted=None if counted is None else torch.tensor(counted, dtype=torch.int32), heads=(Hq, Hkv, D))
+
+
+def _context(c, dev=DEV):
+    return SimpleNamespace(num_reqs=len(c["q_lens"]), cu_q=c["cu"].to(dev), ctx_lens=c["ctx"].to(dev), slot_ids=c["slots"].to(dev),
+                           positions=c["step_positions"].to(dev), q_lens_host=c["q_lens"], ctx_lens_host=c["ctx_lens"],
+                           max_q_len=max(c["q_lens"]))
+
+
+def _rows_on_device(x):
+    """The rows on the device with the stride they have here."""
+    wide = torch.zeros(x.shape[0], x.stride(0), dtype=x.dtype, device=DEV)
+    wide[:, :x.shape[1]] = x.to(DEV)
+    return wide[:, :x.shape[1]]
+
+
+def _gather(c, window=0, in_place=False, **options):
+    Hq, Hkv, D = c["heads"]
+    w = c["weights"].to(DEV)
+    out = w if in_place else torch.full_like(w, -5.0)
+    positions = torch.full(w.shape, -9, dtype=torch.int32, device=DEV)
+    opts = {k: (v.to(DEV) if isinstance(v, torch.Tensor) else v) for k, v in options.items()}
+    ops.accumulate_attention(_rows_on_device(c["qkv"]), c["pages"].to(DEV), c["table"].to(DEV), _context(c), w, out, c.get("scale", D ** -0.5), window,
+                             Hq, Hkv, D, _alloc, positions=positions, counted=None if c["counted"] is None else c["counted"].to(DEV), **opts)
+    torch.cuda.synchronize()
+    return out.cpu(), positions.cpu()
+
+
+def _check_weights(c, window=0, in_place=False, **options):
+    Hq, Hkv, D = c["heads"]
+    got, noted = _gather(c, window, in_place, **options)
+    before = c["weights"] if in_place else torch.full_like(c["weights"], -5.0)
+    want, tol = plain_drafts.gathered(c["qkv"], c["pages"], c["table"], c["cu"], c["ctx"], c["slots"], c["weights"], before,
+                                      c.get("scale", D ** -0.5), window, Hq, Hkv, D, c["counted"], **options)
+    assert torch.isfinite(got).all()
+    over = (got.double() - want).abs() - tol
+    assert float(over.max()) <= 0.0, f"{int((over > 0).sum())} of {over.numel()} entries are off, by {float((got.double() - want).abs().max()):.3e}"
+    for r in range(len(c["q_lens"])):
+        n, k, s = c["q_lens"][r], c["ctx_lens"][r], int(c["slots"][r])
+        a = int(c["cu"][r])
+        assert (noted[s, :, k:k + n] == c["step_positions"][a:a + n]).all()
+        assert (noted[s, :, :k] == -9).all() and (noted[s, :, k + n:] == -9).all()
+    return got
+
+
+LAYOUTS = [(torch.float32, 4, 2, 16, 8), (torch.float32, 6, 2, 80, 24), (torch.bfloat16, 16, 8, 128, 16), (torch.bfloat16, 32, 8, 128, 16),
+           (torch.bfloat16, 12, 1, 96, 32), (torch.bfloat16, 5, 5, 48, 16), (torch.bfloat16, 8, 8, 64, 7), (torch.bfloat16, 7, 1, 20, 16),
+           (torch.bfloat16, 4, 4, 192, 64), (torch.float32, 3, 1, 33, 5), (torch.bfloat16, 40, 2, 256, 16)]
+BATCHES = [([1], [0]), ([1], [77]), ([1, 1, 1], [5, 530, 33]), ([7, 1, 2, 1], [9, 40, 0, 63]), ([40], [25]), ([130, 5], [300, 127]), ([5, 5, 5], [0, 256, 1000])]
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens", BATCHES)
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,P", LAYOUTS)
+def test_accumulate_attention(dtype, Hq, Hkv, D, P, q_lens, ctx_lens):
+    _check_weights(_weights_case(dtype, Hq, Hkv, D, P, q_lens, ctx_lens, Hq + D))
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,P", [(torch.float32, 4, 2, 32, 8), (torch.bfloat16, 16, 4, 128, 16), (torch.bfloat16, 6, 2, 80, 16)])
+@pytest.mark.parametrize("q_lens,ctx_lens", [([1, 3, 1], [700, 65, 1]), ([150, 9], [40, 200])])
+@pytest.mark.parametrize("option", ["window", "window1", "sinks", "softcap", "slopes", "counted", "counted0", "all"])
+def test_accumulate_attention_options(dtype, Hq, Hkv, D, P, q_lens, ctx_lens, option):
+    counted = None
+    if option == "counted":
+        counted = [max(1, n // 2) for n in q_lens]
+    if option in ("counted0", "all"):
+        counted = [0 if i == 1 else n + 5 for i, n in enumerate(q_lens)]
+    c = _weights_case(dtype, Hq, Hkv, D, P, q_lens, ctx_lens, 17, counted=counted)
+    g = torch.Generator().manual_seed(4)
+    options = {}
+    if option in ("sinks", "all"):
+        options["sinks"] = torch.randn(Hq, generator=g) * 2
+    if option in ("softcap", "all"):
+        options["softcap"] = 3.0
+    if option in ("slopes", "all"):
+        options["slopes"] = torch.rand(Hq, generator=g) * 0.2
+    window = {"window": 50, "window1": 1, "all": 33}.get(option, 0)
+    _check_weights(c, window=window, **options)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_accumulate_attention_over_a_latent_cache_and_more_planes(dtype):
+    for planes, Hq, Hkv, D in ((1, 16, 1, 64), (3, 4, 2, 128), (1, 24, 1, 256)):
+        for q_lens, ctx_lens in (([1, 1], [300, 5]), ([60], [100])):
+            _check_weights(_weights_case(dtype, Hq, Hkv, D, 16, q_lens, ctx_lens, planes, planes=planes))
+
+
+def test_accumulate_attention_in_place_and_twice_the_same_bits():
+    for q_lens, ctx_lens in (([1, 1], [600, 90]), ([200], [33])):
+        c = _weights_case(torch.bfloat16, 8, 2, 128, 16, q_lens, ctx_lens, 8)
+        a = _check_weights(c, in_place=True)
+        assert torch.equal(a, _check_weights(c, in_place=True))
+        apart = _check_weights(c)
+        for r in range(len(q_lens)):
+            L, s = q_lens[r] + ctx_lens[r], int(c["slots"][r])
+            assert torch.equal(apart[s, :, :L], a[s, :, :L])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_lens,ctx_lens", [([1], [200]), ([100], [60])])
+def test_accumulate_attention_where_a_page_is_missing_and_garbage_behind_the_end(dtype, q_lens, ctx_lens):
+    """Keys that lie in no page get no weight; NaN in places that no row may see (behind the end, in the future of the rows that count) stays there."""
+    c = _weights_case(dtype, 4, 2, 128, 16, q_lens, ctx_lens, 21)
+    total = q_lens[0] + ctx_lens[0]
+    last = int(c["table"][0, (total - 1) // 16])
+    if total % 16:
+        c["pages"][last, 0, :, total % 16:] = math.nan
+    c["table"][0, 3] = -1
+    _check_weights(c)
+
+
+def test_accumulate_attention_takes_strided_rows_and_large_scores():
+    for q_lens, ctx_lens in (([1, 2], [100, 30]), ([129], [64])):
+        c = _weights_case(torch.bfloat16, 4, 2, 128, 16, q_lens, ctx_lens, 31, std=12.0)
+        wide = torch.zeros(c["qkv"].shape[0], c["qkv"].shape[1] + 24, dtype=torch.bfloat16)
+        wide[:, :c["qkv"].shape[1]] = c["qkv"]
+        c["qkv"] = wide[:, :c["qkv"].shape[1]]
+        _check_weights(c)
+        odd = torch.zeros(c["qkv"].shape[0], c["qkv"].shape[1] + 3, dtype=torch.bfloat16)     # rows off a 16-byte boundary
+        odd[:, :c["qkv"].shape[1]] = c["qkv"]
+        c["qkv"] = odd[:, :c["qkv"].shape[1]]
+        _check_weights(c)
+
+
+def test_accumulate_attention_of_a_long_context():
+    c = _weights_case(torch.bfloat16, 8, 2, 128, 16, [1, 3], [40000, 1], 41)
+    _check_weights(c)
+    c = _weights_case(torch.bfloat16, 4, 1, 128, 64, [700], [3000], 42)
+    _check_weights(c)
+
+
+# ---- eviction ------------------------------------------------------------------------------------------------------------------
+
+def _evict_case(dtype, S, Hkv, D, P, lens, seed, planes=2, coarse=False, ordered=False, extra=2):
+    g = torch.Generator().manual_seed(seed)
+    R = len(lens)
+    blocks = [max(1, -(-n // P)) for n in lens]
+    pages = sum(blocks) + 1
+    order = iter(torch.randperm(pages, generator=g).tolist())
+    table = torch.full((R, max(blocks)), -1, dtype=torch.int32)
+    for r, nb in enumerate(blocks):
+        for b in range(nb):
+            table[r, b] = next(order)
+    cap, slots = max(lens) + extra, R + 1
+    w = torch.exp(1.5 * torch.randn(S, slots, Hkv, cap, generator=g))
+    if coarse:
+        w = w.round()
+    pos = torch.argsort(torch.rand(S, slots, Hkv, cap, generator=g), dim=-1).to(torch.int32)
+    if ordered:
+        pos = torch.arange(cap, dtype=torch.int32).expand(S, slots, Hkv, cap).contiguous()
+    return dict(cache=torch.randn(S, pages, planes, Hkv, P, D, generator=g).to(dtype), table=table,
+                slot_ids=torch.randperm(slots, generator=g)[:R].to(torch.int32), lens=torch.tensor(lens, dtype=torch.int32), weights=w, positions=pos)
+
+
+def _check_evict(c, keep, first, recent, in_place=False):
+    d = {k: v.to(DEV) for k, v in c.items()}
+    wo = d["weights"] if in_place else torch.full_like(d["weights"], -3.0)
+    po = d["positions"] if in_place else torch.full_like(d["positions"], -3)
+    want = plain_drafts.evict(c["cache"], c["table"], c["slot_ids"], c["lens"], c["weights"], c["positions"],
+                              c["weights"] if in_place else wo.cpu(), c["positions"] if in_place else po.cpu(), keep, first, recent)
+    ops.evict_tokens(d["cache"], d["table"], d["slot_ids"], d["lens"], d["weights"], d["positions"], wo, po, keep, first, recent, _alloc)
+    torch.cuda.synchronize()
+    assert torch.equal(po.cpu(), want[2])
+    assert torch.equal(wo.cpu().view(torch.int32), want[1].view(torch.int32))
+    assert torch.equal(d["cache"].cpu().contiguous().view(torch.uint8), want[0].contiguous().view(torch.uint8))
+    return d, wo, po
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("dtype,S,Hkv,D,P,planes", [(torch.bfloat16, 2, 2, 128, 16, 2), (torch.float32, 1, 3, 80, 24, 2), (torch.bfloat16, 2, 1, 33, 5, 1),
+                                                    (torch.bfloat16, 1, 2, 6, 16, 3)])
+@pytest.mark.parametrize("lens,keep,first,recent", [([65], 64, 2, 8), ([300, 17, 64, 63, 1, 0, 65], 64, 3, 20), ([40, 41], 1, 0, 0), ([40, 9], 1, 0, 1),
+                                                    ([100], 33, 0, 33), ([513, 1030], 512, 4, 0), ([700, 3], 1000, 1, 1)])
+def test_evict_tokens(dtype, S, Hkv, D, P, planes, lens, keep, first, recent, in_place):
+    _check_evict(_evict_case(dtype, S, Hkv, D, P, lens, keep + len(lens), planes), keep, first, recent, in_place)
+
+
+def test_evict_tokens_with_equal_weights():
+    _check_evict(_evict_case(torch.bfloat16, 1, 2, 64, 16, [500, 90], 3, coarse=True), 77, 2, 9)
+    c = _evict_case(torch.bfloat16, 1, 2, 64, 16, [500, 90], 4)
+    c["weights"][:] = 0.25
+    _check_evict(c, 77, 2, 9)
+
+
+def test_evict_tokens_with_infinities_and_nan():
+    c = _evict_case(torch.float32, 1, 2, 16, 16, [200, 130], 5)
+    g = torch.Generator().manual_seed(1)
+    m = torch.rand(c["weights"].shape, generator=g)
+    c["weights"][m < 0.2] = math.nan
+    c["weights"][(m >= 0.2) & (m < 0.3)] = math.inf
+    c["weights"][(m >= 0.3) & (m < 0.4)] = -math.inf
+    c["weights"][(m >= 0.4) & (m < 0.5)] = -0.0
+    c["weights"][(m >= 0.5) & (m < 0.6)] = 0.0
+    for keep in (20, 80, 120):
+        d = {k: v.clone() for k, v in c.items()}
+        _check_evict(d, keep, 1, 5)
+
+
+@pytest.mark.parametrize("lens,keep,first,recent", [([9001, 4097, 20], 1000, 4, 100), ([33000], 32999, 4, 64), ([20000, 20000], 15000, 0, 0), ([70001], 128, 2, 32)])
+def test_evict_tokens_from_long_caches(lens, keep, first, recent):
+    for in_place in (False, True):
+        _check_evict(_evict_case(torch.bfloat16, 1, 1, 16, 16, lens, 6, ordered=keep == 1000), keep, first, recent, in_place)
+
+
+def test_evicting_twice_is_evicting_from_what_is_left():
+    c = _evict_case(torch.bfloat16, 2, 2, 64, 16, [300, 200], 9)
+    d, w, p = _check_evict(c, 150, 2, 20, in_place=True)
+    again = dict(cache=d["cache"].cpu(), table=c["table"], slot_ids=c["slot_ids"], lens=torch.tensor([150, 150], dtype=torch.int32),
+                 weights=w.cpu(), positions=p.cpu())
+    _check_evict(again, 40, 2, 20, in_place=True)
+
+
+def test_a_slot_or_a_page_that_is_not_there_is_left_alone():
+    """A slot outside the rows: the request is passed over.  A place without a page: its entry is not moved, the others are."""
+    c = _evict_case(torch.bfloat16, 1, 1, 16, 16, [64, 64], 11)
+    c["slot_ids"][0] = 99
+    d = {k: v.to(DEV) for k, v in c.items()}
+    wo, po = torch.zeros_like(d["weights"]), torch.zeros_like(d["positions"])
+    ops.evict_tokens(d["cache"], d["table"], d["slot_ids"], d["lens"], d["weights"], d["positions"], wo, po, 30, 1, 2, _alloc)
+    mine = c["table"][0].long()
+    assert torch.equal(d["cache"].cpu()[:, mine], c["cache"][:, mine])
+    want = plain_drafts.evict(c["cache"], c["table"][1:], c["slot_ids"][1:], c["lens"][1:], c["weights"], c["positions"], wo.cpu() * 0, po.cpu() * 0, 30, 1, 2)
+    assert torch.equal(po.cpu(), want[2]) and torch.equal(d["cache"].cpu(), want[0])
+
+
+# ---- all three, as a serving program calls them -----------------------------------------------------------------------------------
+
+def test_a_step_that_verifies_gathers_and_evicts():
+    """The counts of the verification say which rows' weights are gathered and how long the caches are; the evicted cache, read by the attention
+    kernel, gives the attention over exactly the entries that stayed."""
+    Hq, Hkv, D, P, keep, first, recent = 4, 2, 128, 16, 100, 2, 10
+    q_lens, ctx_lens = [4, 1, 3, 4], [130, 99, 100, 20]
+    c = _weights_case(torch.bfloat16, Hq, Hkv, D, P, q_lens, ctx_lens, 51)
+    c["positions"] = torch.arange(c["weights"].shape[2], dtype=torch.int32).expand(c["weights"].shape).contiguous()
+    c["step_positions"] = torch.tensor([k + i for n, k in zip(q_lens, ctx_lens) for i in range(n)], dtype=torch.int32)
+    g = torch.Generator().manual_seed(5)
+    N, R, V = sum(q_lens), 4, 300
+    logits = torch.randn(N, V, generator=g) * 2
+    rows = [int(c["cu"][r]) + i for r in range(R) for i in range(q_lens[r] - 1)]
+    dl = logits[rows] + 0.3 * torch.randn(len(rows), V, generator=g)
+    v = dict(logits=logits, draft_tokens=dl.argmax(1).to(torch.int32), draft_logits=dl, row_starts=c["cu"], temperature=torch.tensor([0.7, 0.0, 1.0, 0.9]),
+             top_k=torch.tensor([0, 0, 40, 5], dtype=torch.int32), uniform=torch.rand(N, generator=g))
+    d = {k: x.to(DEV) for k, x in v.items()}
+    tokens, counts = torch.zeros(N, dtype=torch.int32, device=DEV), torch.zeros(R, dtype=torch.int32, device=DEV)
+    ops.verify_drafts(d["logits"], d["draft_tokens"], d["draft_logits"], d["row_starts"], d["temperature"], d["top_k"], d["uniform"], tokens, counts, _alloc)
+    w, pos, cache, ctx = c["weights"].to(DEV), c["positions"].to(DEV), c["pages"].to(DEV)[None], _context(c)
+    want_tokens, want_counts = plain_drafts.verify(**v)
+    assert torch.equal(tokens.cpu(), want_tokens) and torch.equal(counts.cpu(), want_counts)
+    ops.accumulate_attention(c["qkv"].to(DEV), cache[0], c["table"].to(DEV), ctx, w, w, D ** -0.5, 0, Hq, Hkv, D, _alloc, positions=pos, counted=counts)
+    want, tol = plain_drafts.gathered(c["qkv"], c["pages"], c["table"], c["cu"], c["ctx"], c["slots"], c["weights"], c["weights"], D ** -0.5, 0, Hq, Hkv, D, want_counts)
+    assert float(((w.cpu().double() - want).abs() - tol).max()) <= 0
+    lens = ctx.ctx_lens + counts
+    gathered, noted = w.cpu(), pos.cpu()
+    ops.evict_tokens(cache, c["table"].to(DEV), ctx.slot_ids, lens, w[None], pos[None], w[None], pos[None], keep, first, recent, _alloc)
+    left = plain_drafts.evict(c["pages"][None], c["table"], c["slots"], lens.cpu(), gathered[None], noted[None], gathered[None], noted[None], keep, first, recent)
+    assert torch.equal(cache.cpu(), left[0]) and torch.equal(w[None].cpu(), left[1]) and torch.equal(pos[None].cpu(), left[2])
+    # attention of the next token over what is left, against attention over the entries that stayed, in the order of their positions
+    q = torch.randn(R, (Hq + 2 * Hkv) * D, generator=g).to(torch.bfloat16)
+    after = [min(int(n), keep) for n in lens]
+    actx = SimpleNamespace(cu_q=torch.arange(R + 1, dtype=torch.int32, device=DEV), ctx_lens=torch.tensor([n - 1 for n in after], dtype=torch.int32, device=DEV),
+                           attn_plan=None, q_lens_host=[1] * R, ctx_lens_host=[n - 1 for n in after], arena=None, max_q_len=1)
+    plan = ops.plan_attention([1] * R, actx.ctx_lens_host, P, (), torch.bfloat16)
+    actx.attn_plan = {"tiles": torch.tensor(plan["tiles"], dtype=torch.int32, device=DEV)}
+    out = torch.zeros(R, Hq * D, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attention(q.to(DEV), cache[0], c["table"].to(DEV), actx, out, D ** -0.5, 0, Hq, Hkv, D)
+    for r in range(R):
+        s = int(c["slots"][r])
+        for h in range(Hq):
+            kv = h // (Hq // Hkv)
+            stayed = sorted(noted_of for noted_of in left[2][0, s, kv, :after[r]].tolist())
+            blocks = c["table"][r].long()
+            k = torch.stack([c["pages"][blocks[j // P], 0, kv, j % P] for j in stayed]).double()
+            val = torch.stack([c["pages"][blocks[j // P], 1, kv, j % P] for j in stayed]).double()
+            o = torch.softmax((k @ q[r, h * D:(h + 1) * D].double()) * D ** -0.5, 0) @ val
+            # the output is rounded to bfloat16 (half a step), as are the softmax's weights in the kernel
+            assert float((out[r, h * D:(h + 1) * D].cpu().double() - o).abs().max()) <= 2.0 ** -8 * (float(o.abs().max()) + float(val.abs().max()))
+
+
+def test_captured_and_replayed_with_other_inputs():
+    """All three in one graph: the second replay, on other logits, caches and lengths in the same buffers, gives what eager calls give."""
+    Hq, Hkv, D, P, keep = 8, 2, 128, 16, 60
+    q_lens = [3, 3]
+    cases = [_weights_case(torch.bfloat16, Hq, Hkv, D, P, q_lens, ctx, 60 + i, extra=40) for i, ctx in enumerate(([90, 100], [100, 40]))]
+    rnd = [_verify_case(2, [2], 1000, 70 + i, True) for i in range(2)]
+    cap = 143
+
+    def buffers(c, v):
+        t = {k: x.to(DEV) for k, x in v.items()}
+        wide = torch.full((2, 9), -1, dtype=torch.int32)
+        wide[:, :c["table"].shape[1]] = c["table"][:, :9]
+        t.update(qkv=c["qkv"].to(DEV), pages=torch.zeros(20, 2, Hkv, P, D, dtype=torch.bfloat16, device=DEV), table=wide.to(DEV), ctx=c["ctx"].to(DEV),
+                 slots=c["slots"].to(DEV), w=c["weights"][..., :cap].contiguous().to(DEV) if c["weights"].shape[2] >= cap else
+                 torch.nn.functional.pad(c["weights"], (0, cap - c["weights"].shape[2])).to(DEV),
+                 pos=torch.arange(cap, dtype=torch.int32, device=DEV).expand(4, Hkv, cap).contiguous(), at=c["step_positions"].to(DEV))
+        t["pages"][:c["pages"].shape[0]] = c["pages"].to(DEV)
+        t.update(tokens=torch.zeros(6, dtype=torch.int32, device=DEV), counts=torch.zeros(2, dtype=torch.int32, device=DEV), lens=torch.zeros(2, dtype=torch.int32, device=DEV))
+        return t
+
+    def step(t, scratch):
+        it = iter(scratch)
+
+        def alloc(shape, dtype):
+            key = next(it)
+            if scratch[key] is None:
+                scratch[key] = torch.empty(shape, dtype=dtype, device=DEV)
+            return scratch[key]
+        ctx = SimpleNamespace(num_reqs=2, cu_q=cases[0]["cu"].to(DEV) if t.get("cu") is None else t["cu"], ctx_lens=t["ctx"], slot_ids=t["slots"],
+                              positions=t["at"], q_lens_host=q_lens, ctx_lens_host=[90, 100], max_q_len=3)
+        ops.verify_drafts(t["logits"], t["draft_tokens"], t["draft_logits"], t["row_starts"], t["temperature"], t["top_k"], t["uniform"], t["tokens"], t["counts"], alloc)
+        ops.accumulate_attention(t["qkv"], t["pages"], t["table"], ctx, t["w"], t["w"], D ** -0.5, 0, Hq, Hkv, D, alloc, positions=t["pos"], counted=t["counts"])
+        torch.add(t["ctx"], t["counts"], out=t["lens"])
+        ops.evict_tokens(t["pages"][None], t["table"], t["slots"], t["lens"], t["w"][None], t["pos"][None], t["w"][None], t["pos"][None], keep, 2, 9, alloc)
+
+    keys = ("pages", "w", "pos", "tokens", "counts")
+    want = []
+    for c, v in zip(cases, rnd):
+        t = buffers(c, v)
+        step(t, {i: None for i in range(8)})
+        want.append({k: t[k].clone() for k in keys})
+    live, scratch = buffers(cases[0], rnd[0]), {i: None for i in range(8)}
+    live["cu"] = cases[0]["cu"].to(DEV)
+    step(live, scratch)                           # sizes the scratch memory
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(live, scratch)
+    for i in (0, 1, 0):
+        fresh = buffers(cases[i], rnd[i])
+        for k, x in fresh.items():
+            live[k].copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for k in keys:
+            assert torch.equal(live[k], want[i][k]), k
+
+
+def test_on_another_stream_and_two_calls_at_once():
+    """Two calls on two streams, each with scratch memory of its own, and the same on the default stream."""
+    c = [_weights_case(torch.bfloat16, 8, 2, 128, 16, q, k, 80 + i) for i, (q, k) in enumerate((([1, 1], [500, 900]), ([300], [20])))]
+    want = [_gather(x)[0] for x in c]
+    streams = [torch.cuda.Stream() for _ in c]
+    got = []
+    for x, s in zip(c, streams):
+        Hq, Hkv, D = x["heads"]
+        w = x["weights"].to(DEV)
+        out = torch.full_like(w, -5.0)
+        args = (x["qkv"].to(DEV), x["pages"].to(DEV), x["table"].to(DEV), _context(x))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            ops.accumulate_attention(*args, w, out, D ** -0.5, 0, Hq, Hkv, D, _alloc)
+        got.append(out)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b)
+
+
+def test_another_device_is_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_current_device", lambda: 1)
+    c = _verify_case(2, [1], 10, 1)
+    with pytest.raises(ops.KernelRefused, match="current device"):
+        _verify(c)

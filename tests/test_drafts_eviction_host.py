@@ -1,0 +1,107 @@
+"""The refusals of the operators that verify drafts, gather attention weights and evict from the cache: arguments are looked at
+before anything is launched, so they are tested without a GPU."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from qwen_engine_b200 import ops
+from qwen_engine_b200.sampling import Sampler, SamplingParams
+
+
+def _empty(shape, dtype):
+    return torch.empty(shape, dtype=dtype)
+
+
+def _verify_args(**other):
+    N, R, V = 5, 2, 11
+    a = dict(logits=torch.zeros(N, V), draft_tokens=torch.zeros(N - R, dtype=torch.int32), draft_logits=torch.zeros(N - R, V),
+             row_starts=torch.tensor([0, 3, 5], dtype=torch.int32), temperature=torch.ones(R), top_k=torch.zeros(R, dtype=torch.int32),
+             uniform=torch.zeros(N), tokens=torch.zeros(N, dtype=torch.int32), counts=torch.zeros(R, dtype=torch.int32), alloc=_empty)
+    a.update(other)
+    return a
+
+
+@pytest.mark.parametrize("other", [
+    dict(logits=torch.zeros(5, 11, dtype=torch.bfloat16)), dict(logits=torch.zeros(11, 5).T), dict(draft_tokens=torch.zeros(4, dtype=torch.int32)),
+    dict(draft_tokens=torch.zeros(3, dtype=torch.int64)), dict(draft_logits=torch.zeros(3, 12)), dict(draft_logits=torch.zeros(3, 11, dtype=torch.float64)),
+    dict(row_starts=torch.zeros(2, dtype=torch.int32)), dict(temperature=torch.ones(3)), dict(temperature=torch.ones(2, dtype=torch.float64)),
+    dict(top_k=torch.zeros(2)), dict(uniform=torch.zeros(4)), dict(tokens=torch.zeros(4, dtype=torch.int32)), dict(uniform=torch.zeros(10)[::2])])
+def test_verify_drafts_refuses(other):
+    with pytest.raises(ops.KernelRefused):
+        ops.verify_drafts(**_verify_args(**other))
+
+
+def test_operands_on_the_cpu_are_refused():
+    with pytest.raises(ops.ExtensionMissing):
+        ops.verify_drafts(**_verify_args())
+    with pytest.raises(ops.ExtensionMissing):
+        ops.accumulate_attention(**_weights_args())
+    with pytest.raises(ops.ExtensionMissing):
+        ops.evict_tokens(**_evict_args())
+
+
+def _weights_args(**other):
+    R, Hq, Hkv, D, P, slots, cap = 2, 4, 2, 16, 8, 3, 40
+    ctx = SimpleNamespace(num_reqs=R, cu_q=torch.tensor([0, 2, 3], dtype=torch.int32), ctx_lens=torch.tensor([5, 9], dtype=torch.int32),
+                          slot_ids=torch.tensor([0, 2], dtype=torch.int32), positions=torch.zeros(3, dtype=torch.int32),
+                          q_lens_host=[2, 1], ctx_lens_host=[5, 9])
+    a = dict(qkv=torch.zeros(3, (Hq + 2 * Hkv) * D), kv_pages=torch.zeros(6, 2, Hkv, P, D), block_tables=torch.zeros(R, 2, dtype=torch.int32),
+             ctx=ctx, weights=torch.zeros(slots, Hkv, cap), out=torch.zeros(slots, Hkv, cap), scale=0.25, window=0, num_heads=Hq,
+             num_kv_heads=Hkv, head_dim=D, alloc=_empty)
+    a.update(other)
+    return a
+
+
+_ONE = torch.zeros(3 * 2 * 40 + 4)
+
+
+@pytest.mark.parametrize("other", [
+    dict(qkv=torch.zeros(3, 128, dtype=torch.bfloat16)), dict(qkv=torch.zeros(128, 3).T), dict(qkv=torch.zeros(3, 60)), dict(num_heads=5),
+    dict(kv_pages=torch.zeros(6, 2, 3, 8, 16)), dict(kv_pages=torch.zeros(6, 2, 8, 16)), dict(kv_pages=torch.zeros(6, 2, 2, 8, 32)[..., ::2]),
+    dict(block_tables=torch.zeros(2, 2, dtype=torch.int64)), dict(block_tables=torch.zeros(3, 2, dtype=torch.int32)),
+    dict(block_tables=torch.zeros(2, 1, dtype=torch.int32)),                         # 10 tokens in one block of 8
+    dict(weights=torch.zeros(3, 2, 9), out=torch.zeros(3, 2, 9)),                    # ... and in 9 places
+    dict(weights=torch.zeros(3, 2, 40, dtype=torch.float64)), dict(out=torch.zeros(3, 2, 41)),
+    dict(weights=_ONE[:240].view(3, 2, 40), out=_ONE[4:].view(3, 2, 40)),            # they overlap
+    dict(positions=torch.zeros(3, 2, 40)), dict(counted=torch.zeros(3, dtype=torch.int32)), dict(counted=torch.zeros(2)),
+    dict(slopes=torch.zeros(2)), dict(sinks=torch.zeros(4, dtype=torch.float64)), dict(scale=0.0), dict(softcap=-1.0)])
+def test_accumulate_attention_refuses(other):
+    with pytest.raises(ops.KernelRefused):
+        ops.accumulate_attention(**_weights_args(**other))
+
+
+def _evict_args(**other):
+    S, R, Hkv, D, P, slots, cap = 2, 2, 2, 16, 8, 3, 16
+    a = dict(cache=torch.zeros(S, 6, 2, Hkv, P, D), block_tables=torch.zeros(R, 2, dtype=torch.int32), slot_ids=torch.tensor([0, 2], dtype=torch.int32),
+             lens=torch.tensor([12, 16], dtype=torch.int32), weights=torch.zeros(S, slots, Hkv, cap),
+             positions=torch.zeros(S, slots, Hkv, cap, dtype=torch.int32), weights_out=torch.zeros(S, slots, Hkv, cap),
+             positions_out=torch.zeros(S, slots, Hkv, cap, dtype=torch.int32), keep=8, first=1, recent=3, alloc=_empty)
+    a.update(other)
+    return a
+
+
+@pytest.mark.parametrize("other", [
+    dict(cache=torch.zeros(6, 2, 2, 8, 16)), dict(cache=torch.zeros(2, 6, 2, 2, 16, 8).transpose(4, 5)), dict(block_tables=torch.zeros(3, 2, dtype=torch.int32)),
+    dict(slot_ids=torch.zeros(3, dtype=torch.int32)), dict(lens=torch.zeros(2)), dict(weights=torch.zeros(1, 3, 2, 16)),
+    dict(weights=torch.zeros(2, 3, 2, 16, dtype=torch.bfloat16)), dict(positions=torch.zeros(2, 3, 2, 17, dtype=torch.int32)),
+    dict(weights_out=torch.zeros(2, 3, 2, 17)), dict(positions_out=torch.zeros(2, 3, 2, 16)), dict(keep=0), dict(first=-1), dict(recent=-1),
+    dict(keep=8, first=5, recent=4)])
+def test_evict_tokens_refuses(other):
+    with pytest.raises(ops.KernelRefused):
+        ops.evict_tokens(**_evict_args(**other))
+
+
+def test_the_sampler_refuses_lists_that_do_not_fit():
+    s = Sampler("cpu")
+    p = [SamplingParams(temperature=1.0)] * 2
+    for drafts, uniforms, rows in [([[1]], [[0.1, 0.2]], 2), ([[1], []], [[0.1, 0.2], []], 3), ([[1], []], [[0.1, 0.2], [0.3]], 4)]:
+        with pytest.raises(ValueError):
+            s.verify(torch.zeros(rows, 9), p, drafts, uniforms)
+
+
+def test_parts_of_rows():
+    """Rows that fill the SMs are not cut; a few rows are cut into as many parts of 256 keys as give every SM two CTAs."""
+    assert ops._attention_weights_parts(64, 8, 1, 4096) == 1
+    assert ops._attention_weights_parts(1, 8, 1, 4096) == 16 and ops._attention_weights_parts(1, 8, 1, 131072) == 37
+    assert ops._attention_weights_parts(1, 1, 1, 1 << 20) == ops.ATTENTION_WEIGHTS_MAX_PARTS and ops._attention_weights_parts(1, 1, 1, 1) == 1
