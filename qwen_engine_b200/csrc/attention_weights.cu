@@ -70,14 +70,14 @@ __device__ __forceinline__ void aw_products(const AwArgs& A, const AwReq& R, int
 
 template <typename T>
 __global__ void __launch_bounds__(AW_THREADS)
-attention_weights_rows_kernel(AwArgs A) {
+attention_weights_rows_kernel(AwArgs A, int few_rows) {
   __shared__ AwTile sm;
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.z, c = blockIdx.y, tile = blockIdx.x / A.parts, part = blockIdx.x - tile * A.parts;
   const AwReq R = aw_req(A, r);
   const int G = A.Hq / A.Hkv, rho0 = tile * AW_TILE, rows = R.counted * G;
-  if (rho0 >= rows) return;
+  if (rho0 >= rows || (long)R.n * G <= few_rows) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   // the tile's keys, and this part's share of their tiles
   const int first = R.ctx + rho0 / G, last = R.ctx + (min(rho0 + AW_TILE, rows) - 1) / G;
@@ -137,7 +137,7 @@ attention_weights_rows_kernel(AwArgs A) {
 
 template <typename T>
 __global__ void __launch_bounds__(AW_THREADS)
-attention_weights_keys_kernel(AwArgs A) {
+attention_weights_keys_kernel(AwArgs A, int few_rows) {
   __shared__ AwTile sm;
   __shared__ float2 row[AW_TILE];
   __shared__ float sums[16][AW_PITCH];
@@ -146,8 +146,9 @@ attention_weights_keys_kernel(AwArgs A) {
   const int r = blockIdx.z, c = blockIdx.y, key0 = blockIdx.x * AW_TILE;
   const AwReq R = aw_req(A, r);
   const int slot = A.slot_ids[r];
-  if (key0 >= R.total || slot < 0 || slot >= A.slots) return;
-  const int G = A.Hq / A.Hkv, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int G = A.Hq / A.Hkv;
+  if (key0 >= R.total || slot < 0 || slot >= A.slots || (few_rows >= 0 && (long)R.n * G <= few_rows)) return;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   // the rows that see any of these keys
   const int t0 = max(0, key0 - R.ctx);
   const int t1 = A.window > 0 ? (int)min((long)R.counted, (long)key0 + AW_TILE - 1 + A.window - R.ctx) : R.counted;
@@ -196,12 +197,13 @@ attention_weights_keys_kernel(AwArgs A) {
   }
 }
 
+// few_rows: requests of at most so many rows (a query token x a query head of a kv head's group) are left to another kernel (-1: none).
 extern "C" int qe_attention_weights(const void* q, long q_stride, int T, const void* pages, int num_pages, int planes,
                                     const int* block_tables, int max_blocks, const int* cu_q, const int* ctx_lens, const int* slot_ids,
                                     const int* counted, const int* step_positions, int* positions, const float* weights, float* out,
                                     int slots, long capacity, int R, int Hq, int Hkv, int D, int page, int window, float scale,
                                     float softcap, const float* slopes, const float* sinks, float* stats, int parts, int max_q, int max_total,
-                                    int dtype, cudaStream_t stream) {
+                                    int few_rows, int dtype, cudaStream_t stream) {
   if (R <= 0 || max_total <= 0) return 0;
   if (Hkv < 1 || Hq % Hkv || D < 1 || page < 1) QE_REFUSE("attention_weights: heads %d/%d, head_dim %d, pages of %d", Hq, Hkv, D, page);
   if (R > 65535 || Hkv > 65535) QE_REFUSE("attention_weights: %d requests, %d kv heads are more than a launch takes", R, Hkv);
@@ -212,11 +214,11 @@ extern "C" int qe_attention_weights(const void* q, long q_stride, int T, const v
   if (row_tiles * parts > 0x7fffffffL) QE_REFUSE("attention_weights: %d rows are more than a launch takes", max_q);
   const dim3 grid_rows((unsigned)(row_tiles * parts), (unsigned)Hkv, (unsigned)R), grid_keys((unsigned)key_tiles, (unsigned)Hkv, (unsigned)R);
   if (dtype == QE_DTYPE_F32) {
-    if (row_tiles > 0) qe_launch(attention_weights_rows_kernel<float>, grid_rows, dim3(AW_THREADS), 0, stream, A);
-    qe_launch(attention_weights_keys_kernel<float>, grid_keys, dim3(AW_THREADS), 0, stream, A);
+    if (row_tiles > 0) qe_launch(attention_weights_rows_kernel<float>, grid_rows, dim3(AW_THREADS), 0, stream, A, few_rows);
+    qe_launch(attention_weights_keys_kernel<float>, grid_keys, dim3(AW_THREADS), 0, stream, A, few_rows);
   } else {
-    if (row_tiles > 0) qe_launch(attention_weights_rows_kernel<__nv_bfloat16>, grid_rows, dim3(AW_THREADS), 0, stream, A);
-    qe_launch(attention_weights_keys_kernel<__nv_bfloat16>, grid_keys, dim3(AW_THREADS), 0, stream, A);
+    if (row_tiles > 0) qe_launch(attention_weights_rows_kernel<__nv_bfloat16>, grid_rows, dim3(AW_THREADS), 0, stream, A, few_rows);
+    qe_launch(attention_weights_keys_kernel<__nv_bfloat16>, grid_keys, dim3(AW_THREADS), 0, stream, A, few_rows);
   }
   QE_CHECK_LAUNCH("attention_weights");
   return 0;

@@ -1695,6 +1695,28 @@ def _attention_weights_parts(row_tiles: int, heads: int, requests: int, max_tota
     return max(1, min(-(-FLASH_TARGET_CTAS // max(1, row_tiles * heads * requests)), -(-max_total // 256), ATTENTION_WEIGHTS_MAX_PARTS))
 
 
+ATTENTION_WEIGHTS_FEW_ROWS = 32               # rows of a request (a query token x a query head of a kv head's group) up to which the kernel of few rows serves
+ATTENTION_WEIGHTS_CLUSTER_SMEM = 110 * 1024   # bytes of scores up to which a request's rows and keys are shared by a cluster: two CTAs an SM
+
+
+def attention_weights_cluster(rows: int, heads: int, head_dim: int, requests: int, span: int) -> tuple[int, int]:
+    """(CTAs of a cluster, keys a CTA) for the gathered weights of a few rows, (0, 0) where scratch memory holds the scores: as many
+    of 1, 2, 4, 8 CTAs as give every SM two."""
+    ctas = 1
+    while ctas < 8 and (requests * heads * ctas < FLASH_TARGET_CTAS or _cluster_smem(rows, head_dim, -(-span // ctas)) > ATTENTION_WEIGHTS_CLUSTER_SMEM):
+        ctas *= 2
+    part = -(-span // (32 * ctas)) * 32
+    if _cluster_smem(rows, head_dim, part) > ATTENTION_WEIGHTS_CLUSTER_SMEM:
+        return 0, 0
+    return ctas, part
+
+
+def _cluster_smem(rows: int, head_dim: int, part: int) -> int:
+    """Shared memory of a CTA of that kernel: the queries as fragments, and its keys' scores."""
+    lc = 2 if head_dim <= 64 else 4
+    return (2 if rows > 16 else 1) * -(-head_dim // (32 * lc)) * lc * 1024 + rows * (part + 4) * 4
+
+
 def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables: torch.Tensor, ctx, weights: torch.Tensor,
                          out: torch.Tensor, scale: float, window: int, num_heads: int, num_kv_heads: int, head_dim: int, alloc,
                          positions: Optional[torch.Tensor] = None, counted: Optional[torch.Tensor] = None,
@@ -1740,15 +1762,31 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
     _here("accumulate_attention", qkv, kv_pages, block_tables, weights, out, positions, counted, slopes, sinks, ctx.cu_q)
     if R == 0 or T == 0:
         return
-    max_q, max_total = max(ctx.q_lens_host), min(int(weights.shape[2]), int(block_tables.shape[1]) * page)
-    parts = _attention_weights_parts(-(-max_q * (Hq // Hkv) // 64), Hkv, R, max_total)
-    stats = alloc((T * Hq, parts, 2), torch.float32)
-    _check(lib().qe_attention_weights(
-        _ptr(qkv), ctypes.c_long(qkv.stride(0)), T, _ptr(kv_pages), int(kv_pages.shape[0]), planes, _ptr(block_tables),
-        int(block_tables.shape[1]), _ptr(ctx.cu_q), _ptr(ctx.ctx_lens), _ptr(ctx.slot_ids), _ptr(counted), _ptr(ctx.positions),
-        _ptr(positions), _ptr(weights), _ptr(out), int(weights.shape[0]), ctypes.c_long(weights.shape[2]), R, Hq, Hkv, D, page,
-        int(window), ctypes.c_float(scale), ctypes.c_float(softcap), _ptr(slopes), _ptr(sinks), _ptr(stats), parts, max_q, max_total,
-        _dt(qkv), _stream()), "accumulate_attention")
+    max_total = min(int(weights.shape[2]), int(block_tables.shape[1]) * page)
+    G = Hq // Hkv
+    args = (_ptr(qkv), ctypes.c_long(qkv.stride(0)), T, _ptr(kv_pages), int(kv_pages.shape[0]), planes, _ptr(block_tables),
+            int(block_tables.shape[1]), _ptr(ctx.cu_q), _ptr(ctx.ctx_lens), _ptr(ctx.slot_ids), _ptr(counted), _ptr(ctx.positions),
+            _ptr(positions), _ptr(weights), _ptr(out), int(weights.shape[0]), ctypes.c_long(weights.shape[2]), R, Hq, Hkv, D, page,
+            int(window), ctypes.c_float(scale), ctypes.c_float(softcap), _ptr(slopes), _ptr(sinks))
+    # the requests of a few rows, and the others
+    few = -1
+    if qkv.dtype == torch.bfloat16 and D % 8 == 0 and D <= 1024 and kv_pages.data_ptr() % 16 == 0:
+        few = max((n * G for n in ctx.q_lens_host if n * G <= ATTENTION_WEIGHTS_FEW_ROWS), default=-1)
+    if few > 0:
+        span = min(max_total, int(window) + few // G + 31) if window > 0 else max_total
+        ctas, part_keys = attention_weights_cluster(few, Hkv, D, R, span)
+        scores, ld, parts, stats = None, 0, 1, None
+        if ctas == 0:
+            parts = _attention_weights_parts(1, Hkv, R, span)
+            ld = -(-(span + 32) // 32) * 32
+            scores, stats = alloc((R, Hkv, few, ld), torch.float32), alloc((T * Hq, parts, 2), torch.float32)
+        _check(lib().qe_attention_weights_few(*args, _ptr(stats), parts, few, max_total, span, ctas, part_keys, _ptr(scores), ctypes.c_long(ld), _stream()),
+               "accumulate_attention")
+    max_q = max(ctx.q_lens_host)
+    if few < max_q * G:
+        parts = _attention_weights_parts(-(-max_q * G // 64), Hkv, R, max_total)
+        stats = alloc((T * Hq, parts, 2), torch.float32)
+        _check(lib().qe_attention_weights(*args, _ptr(stats), parts, max_q, max_total, few, _dt(qkv), _stream()), "accumulate_attention")
 
 
 def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,
