@@ -884,7 +884,7 @@ class DeviceWaitTimeout(RuntimeError):
 
 _STATUS_WORDS = ("qe_gemm_tc", "qe_gemm_tc_swap", "qe_gemm_tc_pair", "qe_gemm_tc_splitk", "qe_gemm_tc_stream", "qe_flash_attention_tc",
                  "qe_flash_attention", "qe_decode_attention_mma", "qe_small_m", "qe_latent_decode", "qe_moe_tc", "qe_latent_attention_tc",
-                 "qe_head_linear_tc")
+                 "qe_head_linear_tc", "qe_attention_weights_tc")
 
 
 def device_status() -> dict[str, int]:
@@ -1711,6 +1711,14 @@ def attention_weights_cluster(rows: int, heads: int, head_dim: int, requests: in
     return ctas, part
 
 
+ATTENTION_WEIGHTS_TC = True                   # more rows in bfloat16: the kernels on the tensor cores (False: the general kernels serve them)
+
+
+def attention_weights_tc_parts(units: int, tiles: int) -> int:
+    """In how many parts each unit's walk over ``tiles`` tiles is cut: four units an SM, four tiles a part at least."""
+    return max(1, min(-(-4 * TC_TARGET_CTAS // max(1, units)), -(-tiles // 4), ATTENTION_WEIGHTS_MAX_PARTS))
+
+
 def _cluster_smem(rows: int, head_dim: int, part: int) -> int:
     """Shared memory of a CTA of that kernel: the queries as fragments, and its keys' scores."""
     lc = 2 if head_dim <= 64 else 4
@@ -1783,7 +1791,19 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
         _check(lib().qe_attention_weights_few(*args, _ptr(stats), parts, few, max_total, span, ctas, part_keys, _ptr(scores), ctypes.c_long(ld), _stream()),
                "accumulate_attention")
     max_q = max(ctx.q_lens_host)
-    if few < max_q * G:
+    if few >= max_q * G:
+        return
+    if (ATTENTION_WEIGHTS_TC and qkv.dtype == torch.bfloat16 and qkv.data_ptr() % 16 == 0 and qkv.stride(0) % 8 == 0
+            and kv_pages.data_ptr() % 16 == 0 and lib().qe_attention_weights_tc_supported(Hq, Hkv, D, page)):
+        tpt, na = 128 // G, 4 if D <= 128 else (2 if D <= 192 else 1)      # tokens of a tile of queries, tiles a unit
+        many = [(n, n + c) for n, c in zip(ctx.q_lens_host, ctx.ctx_lens_host) if n * G > few]
+        parts1 = attention_weights_tc_parts(sum(-(-n // (tpt * na)) for n, _ in many) * Hkv, -(-max_total // 128))
+        parts2 = attention_weights_tc_parts(sum(-(-t // (128 * na)) for _, t in many) * Hkv, -(-max_q // tpt))
+        stats, merged = alloc((T * Hq, parts1, 2), torch.float32), alloc((2, Hkv, T // tpt + R, 128), torch.float32)
+        sums = alloc((parts2, R, Hkv, max_total), torch.float32) if parts2 > 1 else None
+        _check(lib().qe_attention_weights_tc(*args, _ptr(stats), parts1, parts2, _ptr(merged), _ptr(sums), max_q, max_total, few, _stream()),
+               "accumulate_attention")
+    else:
         parts = _attention_weights_parts(-(-max_q * G // 64), Hkv, R, max_total)
         stats = alloc((T * Hq, parts, 2), torch.float32)
         _check(lib().qe_attention_weights(*args, _ptr(stats), parts, max_q, max_total, few, _dt(qkv), _stream()), "accumulate_attention")

@@ -557,3 +557,28 @@ def test_another_device_is_refused(monkeypatch):
     c = _verify_case(2, [1], 10, 1)
     with pytest.raises(ops.KernelRefused, match="current device"):
         _verify(c)
+
+
+# ---- which kernels served ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(32, 8, 128, 16), (5, 5, 48, 16), (12, 1, 96, 24), (4, 4, 192, 64), (6, 3, 256, 8), (128, 1, 64, 128), (7, 1, 8, 16)])
+@pytest.mark.parametrize("q_lens,ctx_lens", [([33], [0]), ([129, 1, 700], [1, 300, 257]), ([1100, 260], [900, 0])])
+def test_accumulate_attention_on_the_tensor_cores_and_without(Hq, Hkv, D, P, q_lens, ctx_lens, monkeypatch):
+    """Portions of many rows through both kernels that take them, units of one to four tiles, odd numbers of tiles, several parts; no wait ran out."""
+    c = _weights_case(torch.bfloat16, Hq, Hkv, D, P, q_lens, ctx_lens, 90)
+    before = ops.launch_count
+    a = _check_weights(c)
+    assert ops.device_status() == {}
+    assert torch.equal(a, _check_weights(c))
+    monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_TC", False)
+    _check_weights(c)
+    assert ops.launch_count > before
+
+
+def test_accumulate_attention_on_the_tensor_cores_with_every_option():
+    for q_lens, ctx_lens in (([300, 90], [500, 3]), ([64], [0])):
+        for Hq, Hkv in ((8, 2), (6, 2), (3, 3)):
+            c = _weights_case(torch.bfloat16, Hq, Hkv, 64, 16, q_lens, ctx_lens, 91, counted=[q_lens[0] - 7] + [0] * (len(q_lens) - 1))
+            _check_weights(c, window=100, sinks=torch.randn(Hq), softcap=4.0, slopes=torch.rand(Hq) * 0.1)
+            _check_weights(c, window=1, sinks=torch.randn(Hq))
+            _check_weights(c, window=129, in_place=True)
