@@ -6,22 +6,25 @@
 // keys in the second) and streams tiles of 128 rows of the other (B) past them, 128 x 128 products S = A B^T by
 // tcgen05.mma into one of four accumulators of tensor memory.  A thread owns a row of A (= a lane of tensor memory): its
 // running maximum and sum over the columns in the first pass, its sum in the second; nothing is exchanged between threads but at
-// the end.  Four tiles of A a tile of B keep the reads from L2 at 8 KB a product.  Ten warps: two groups of four read accumulators
-// (products alternate between them), one fetches tiles with TMA, one issues the products.
+// the end.  Four tiles of A a tile of B keep the reads from L2 at 8 KB a product.  Eighteen warps: four groups of four read one accumulator
+// each, one warp fetches tiles with TMA, one issues the products.
 //
 // A unit is a (request, kv head, group of A tiles) and a part of the B tiles; parts are merged by a small kernel behind each
-// pass, in their order, so sums do not depend on which CTA was first.  Between the passes it leaves every row's -maximum
-// and 1 / sum in the order of the second pass's columns.
+// pass, in their order, so sums do not depend on which CTA was first.  Between the passes it leaves -log2 of every row's whole
+// sum, exponentials and maximum together, in the order of the second pass's columns: a weight is then one exponential.
 //
 // What bounds it: a product of 128 x 128 x 128 takes the tensor cores 512 cycles and its 16 384 exponentials the
-// special-function unit 1 024.
+// special-function unit 1 024.  So a quarter of the exponentials is a polynomial (at2_poly2), two at a time on the float32 units: more
+// of them cost the readers more instructions than the special-function unit gains.
 //
 // Every wait is bounded: one that runs out records a code, raises the CTA's abort flag, and the CTA leaves without writing.
 #include "attention_weights.cuh"
 #include "tcgen05.cuh"
 
 #define AT2_TILE 128
-#define AT2_THREADS 320
+#define AT2_GROUPS 4                              // groups of four warps that read accumulators, one each
+#define AT2_READERS (128 * AT2_GROUPS)
+#define AT2_THREADS (AT2_READERS + 64)
 #define AT2_BLOCK_BYTES (AT2_TILE * 128)         // 64 channels of a tile: 128-byte swizzled rows
 #define AT2_BLOCKS 12                            // such blocks in shared memory
 #define AT2_MAX_RING 4
@@ -34,7 +37,8 @@ struct __align__(1024) AwTcSmem {
   uint64_t a_full, b_full[AT2_MAX_RING], b_empty[AT2_MAX_RING], s_full[4], s_empty[4];
   uint32_t tmem_base;
   int abort_flag, missing;
-  float2 meet[AT2_TILE];
+  float2 meet[AT2_GROUPS][AT2_TILE];
+  float4 negl[4 * AT2_GROUPS][2][32];            // second pass: a tile's columns' values for each warp, two tiles in turn
 };
 
 struct AwTc {
@@ -42,8 +46,8 @@ struct AwTc {
   int tpt;                     // tokens of a tile of queries
   int kb, na, ring;            // 64-channel blocks of a tile, A tiles of a unit at most (1, 2, 4), B tiles in flight
   int box, parts;              // keys of a TMA box; parts of a unit's B tiles
-  int tiles;                   // rows of `negm` and `inv` for a kv head: tiles of queries of all requests
-  float* negm; float* inv;     // [Hkv, tiles, 128]: first pass's result, for the second
+  int tiles;                   // rows of `negl` for a kv head: tiles of queries of all requests
+  float* negl;                 // [Hkv, tiles, 128]: first pass's result, for the second
   float* sums; long sums_ld;   // [parts, R, Hkv, sums_ld]: second pass's parts (null: it writes the output)
 };
 
@@ -73,79 +77,96 @@ __device__ __forceinline__ void at2_wait_ld(uint32_t (&u)[32]) {
 // where request r's tiles of queries begin among all requests' (a tile never holds two requests' rows)
 __device__ __forceinline__ int at2_tile0(const AwReq& R, int r, int tpt) { return R.row0 / tpt + r; }
 
+// 2^x of two x <= 0 (or a little above) without the special-function unit: x = n + f, |f| <= 1/2, 2^f by a polynomial of degree 5 that is 1 at 0 and
+// whose largest relative error on the interval is least (fitted by weighted least squares; 1.6 10^-7 with its float32 coefficients), n into the exponent.
+__device__ __forceinline__ float2 at2_poly2(float2 x) {
+  x.x = fmaxf(x.x, -127.f); x.y = fmaxf(x.y, -127.f);           // (there n = -127 and f = 0 give the bits of 0; between that and -126.5 f > 0 gives a subnormal)
+  const float magic = 12582912.f;                              // 1.5 2^23: the sum's low bits are x rounded to an integer
+  const float2 t = at2_add(x, make_float2(magic, magic)), n = at2_add(t, make_float2(-magic, -magic));
+  const float2 f = at2_fma(n, make_float2(-1.f, -1.f), x);
+  float2 p = make_float2(0.001326472731307149f, 0.001326472731307149f);
+  p = at2_fma(p, f, make_float2(0.009671512991189957f, 0.009671512991189957f));
+  p = at2_fma(p, f, make_float2(0.05550733581185341f, 0.05550733581185341f));
+  p = at2_fma(p, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
+  p = at2_fma(p, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
+  p = at2_fma(p, f, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+// whether the pair of columns 2 j, 2 j + 1 of a chunk goes there
+__device__ constexpr bool at2_on_poly(int j) { return (j & 3) == 1; }
+__device__ __forceinline__ float2 at2_exp2(float2 x, bool poly) { return poly ? at2_poly2(x) : make_float2(at2_ex2(x.x), at2_ex2(x.y)); }
+
 // one thread's share of the first pass: its row's running maximum and sum, and the keys it may see
 struct At2Row { float m, z, slope; int lo, hi, pos; };
 
 // 32 scores of the row, columns c0 .. c0 + 31 of the key tile that starts at key `base`
 template <bool GENERAL>
-__device__ __forceinline__ void at2_row_chunk(const AwArgs& A, const AwReq& R, int r, const uint32_t (&u)[32], int base, int c0, At2Row& st, bool missing) {
+__device__ __forceinline__ void at2_row_chunk(const AwArgs& A, int r, uint32_t (&u)[32], int base, int c0, At2Row& st, bool missing) {
   const int k0 = base + c0;
   const bool in = k0 >= st.lo && k0 + 32 <= st.hi && !missing, out = k0 >= st.hi || k0 + 32 <= st.lo;
   if (__all_sync(0xffffffffu, out)) return;
-  float v[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
   if (GENERAL) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = aw_score(A, v[i], st.slope, st.pos - (k0 + i));
+    for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(aw_score(A, __uint_as_float(u[i]), st.slope, st.pos - (k0 + i)));
   }
   const float sc = GENERAL ? 1.f : A.scale * AW_LOG2E;
   if (!__all_sync(0xffffffffu, in)) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const int key = k0 + i;
-      v[i] = key >= st.lo && key < st.hi ? v[i] : -INFINITY;
-    }
-    if (missing) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = aw_page(A, r, k0 + i) >= 0 ? v[i] : -INFINITY;
+      if (!(key >= st.lo && key < st.hi) || (missing && aw_page(A, r, key) < 0)) u[i] = 0xff800000u;      // -inf
     }
   }
-  float ma = at2_max3(v[0], v[1], v[2]), mb = at2_max3(v[3], v[4], v[5]);
+  float ma = at2_max3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
+  float mb = at2_max3(__uint_as_float(u[3]), __uint_as_float(u[4]), __uint_as_float(u[5]));
 #pragma unroll
-  for (int i = 6; i < 30; i += 4) { ma = at2_max3(ma, v[i], v[i + 1]); mb = at2_max3(mb, v[i + 2], v[i + 3]); }
-  const float mx = fmaxf(st.m, at2_max3(ma, mb, fmaxf(v[30], v[31])) * sc);      // (the scale is positive)
+  for (int i = 6; i < 30; i += 4) {
+    ma = at2_max3(ma, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+    mb = at2_max3(mb, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
+  }
+  const float mx = fmaxf(st.m, at2_max3(ma, mb, fmaxf(__uint_as_float(u[30]), __uint_as_float(u[31]))) * sc);      // (the scale is positive)
   const float nb = mx == -INFINITY ? 0.f : -mx;
   const float2 sc2 = make_float2(sc, sc), nb2 = make_float2(nb, nb);
   float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
-    const float2 x = at2_fma(make_float2(v[i], v[i + 1]), sc2, nb2), y = at2_fma(make_float2(v[i + 2], v[i + 3]), sc2, nb2);
-    s0 = at2_add(s0, make_float2(at2_ex2(x.x), at2_ex2(x.y)));
-    s1 = at2_add(s1, make_float2(at2_ex2(y.x), at2_ex2(y.y)));
+  for (int j = 0; j < 16; ++j) {
+    const float2 x = at2_fma(make_float2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])), sc2, nb2);
+    const float2 e = at2_exp2(x, at2_on_poly(j));
+    if (j & 1) s1 = at2_add(s1, e); else s0 = at2_add(s0, e);
   }
   st.z = st.z * at2_ex2(st.m + nb) + ((s0.x + s0.y) + (s1.x + s1.y));
   st.m = mx;
 }
 
-// The second pass's: 32 columns (rows of queries) of the thread's key; lo, hi: the columns that see it; nm, iv: the columns' -maximum and 1 / sum.
+// The second pass's: 32 columns (rows of queries) of the thread's key; lo, hi: the columns that see it; nl: the columns' values (shared memory).
 template <bool GENERAL>
-__device__ __forceinline__ void at2_key_chunk(const AwArgs& A, const uint32_t (&u)[32], int c0, int lo, int hi, const float* nm, const float* iv,
-                                              int c, int G, int dist0, float2& acc) {
+__device__ __forceinline__ void at2_key_chunk(const AwArgs& A, uint32_t (&u)[32], int c0, int lo, int hi, const float* nl, int c, int G,
+                                              int dist0, float2& acc) {
   const bool in = c0 >= lo && c0 + 32 <= hi, out = c0 >= hi || c0 + 32 <= lo;
   if (__all_sync(0xffffffffu, out)) return;
-  const bool whole = __all_sync(0xffffffffu, in);
   const float sc = GENERAL ? 1.f : A.scale * AW_LOG2E;
+  if (GENERAL) {
+    int t = c0 / G, g = c0 - t * G;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      u[i] = __float_as_uint(aw_score(A, __uint_as_float(u[i]), A.slopes ? A.slopes[c * G + g] : 0.f, dist0 + t));
+      if (++g == G) { g = 0; ++t; }
+    }
+  }
+  if (!__all_sync(0xffffffffu, in)) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c0 + i < lo || c0 + i >= hi) u[i] = 0xff800000u;      // -inf
+  }
   const float2 sc2 = make_float2(sc, sc);
   float2 a0 = make_float2(0.f, 0.f), a1 = a0;
-  int t = 0, g = 0;
-  if (GENERAL) { t = c0 / G; g = c0 - t * G; }
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = __uint_as_float(u[i + e]);
-      if (GENERAL) {
-        v[e] = aw_score(A, v[e], A.slopes ? A.slopes[c * G + g] : 0.f, dist0 + t);
-        if (++g == G) { g = 0; ++t; }
-      }
-      if (!whole) v[e] = c0 + i + e >= lo && c0 + i + e < hi ? v[e] : -INFINITY;
-    }
-    const float4 m4 = __ldg(reinterpret_cast<const float4*>(nm + c0 + i)), i4 = __ldg(reinterpret_cast<const float4*>(iv + c0 + i));
-    const float2 x = at2_fma(make_float2(v[0], v[1]), sc2, make_float2(m4.x, m4.y)), y = at2_fma(make_float2(v[2], v[3]), sc2, make_float2(m4.z, m4.w));
-    a0 = at2_fma(make_float2(at2_ex2(x.x), at2_ex2(x.y)), make_float2(i4.x, i4.y), a0);
-    a1 = at2_fma(make_float2(at2_ex2(y.x), at2_ex2(y.y)), make_float2(i4.z, i4.w), a1);
+  for (int j = 0; j < 16; j += 2) {
+    const float4 l4 = *(reinterpret_cast<const float4*>(nl + c0) + (j >> 1));
+    const float2 x = at2_fma(make_float2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])), sc2, make_float2(l4.x, l4.y));
+    const float2 y = at2_fma(make_float2(__uint_as_float(u[2 * j + 2]), __uint_as_float(u[2 * j + 3])), sc2, make_float2(l4.z, l4.w));
+    a0 = at2_add(a0, at2_exp2(x, at2_on_poly(j)));
+    a1 = at2_add(a1, at2_exp2(y, at2_on_poly(j + 1)));
   }
   acc = at2_add(acc, at2_add(a0, a1));
 }
@@ -202,7 +223,7 @@ attention_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     sm.missing = 0;
     mbar_init_fence();
   }
-  if (work && warp == 9) tc_alloc(&sm.tmem_base, AT2_COLS);
+  if (work && warp == 4 * AT2_GROUPS + 1) tc_alloc(&sm.tmem_base, AT2_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -215,7 +236,7 @@ attention_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     __syncthreads();
   }
 
-  if (warp == 8) {
+  if (warp == 4 * AT2_GROUPS) {
     // ================= fetching ============================================================================
     if (work) {
       auto fetch_q = [&](unsigned char* dst, int tile, uint64_t* bar) {
@@ -257,136 +278,142 @@ attention_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
           for (uint32_t i = 0; i < TC_WAIT_LIMIT; ++i) if (mbar_try_wait(&sm.b_full[s % n_ring], (s / n_ring) & 1)) break;
       }
     }
-  } else if (warp == 9) {
-    // ================= products: one thread ==================================================================
-    if (work && lane == 0) {
+  } else if (warp == 4 * AT2_GROUPS + 1) {
+    // ================= products ================================================================================
+    // The whole warp walks the loop and one lane is elected for each instruction (tcgen05.cuh says why); with the descriptors worked
+    // out beside the loop.  (One lane in a branch, descriptors worked out in the loop: 180 cycles an instruction, and the readers waited.)
+    if (work) {
       constexpr uint32_t idesc = make_idesc(AT2_TILE, AT2_TILE);
       const int ks = (A.D + 15) / 16;
-      bool ok = mbar_wait(&sm.a_full, 0, abort_flag, 2, &g_awtc_status);
-      for (int s = 0; ok && s < steps; ++s) {
-        const int st = s % n_ring;
-        ok = mbar_wait(&sm.b_full[st], (s / n_ring) & 1, abort_flag, 3, &g_awtc_status);
-        for (int a = 0; ok && a < n_a; ++a) {
-          const int i = s * n_seq + a, acc = i & 3;
-          if (i >= 4) ok = mbar_wait(&sm.s_empty[acc], ((i >> 2) - 1) & 1, abort_flag, 4, &g_awtc_status);
+      const uint64_t d0 = make_smem_desc(smem_u32(sm.tiles[0]));
+      const uint32_t tile_step = (uint32_t)tile_blocks * (AT2_BLOCK_BYTES >> 4);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&sm.a_full, 0, abort_flag, 2, &g_awtc_status));
+      int st = 0, i = 0;
+      uint32_t b_par = 0;
+      for (int s = 0; ok && s < steps; ++s, i += n_seq) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[st], b_par, abort_flag, 3, &g_awtc_status));
+        const uint64_t db = d0 + (uint32_t)(C.na + st) * tile_step;
+        uint64_t da = d0;
+        for (int a = 0; ok && a < n_a; ++a, da += tile_step) {
+          const int acc = (i + a) & 3, use = (i + a) >> 2;
+          if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm.s_empty[acc], (use - 1) & 1, abort_flag, 4, &g_awtc_status));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = make_smem_desc(smem_u32(a_tile(a))), db = make_smem_desc(smem_u32(b_tile(st)));
-          for (int k = 0; k < ks; ++k) {
-            const uint64_t off = (uint64_t)(k >> 2) * (AT2_BLOCK_BYTES >> 4) + 2 * (k & 3);
-            tc_mma_bf16(tmem + acc * AT2_TILE, da + off, db + off, idesc, k != 0);
+          const uint32_t d = tmem + acc * AT2_TILE;
+          if (ks == 8) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = (uint32_t)(k >> 2) * (AT2_BLOCK_BYTES >> 4) + 2 * (k & 3);
+              tc_mma_bf16_elect(d, da + off, db + off, idesc, k != 0);
+            }
+          } else {
+            for (int k = 0; k < ks; ++k) {
+              const uint32_t off = (uint32_t)(k >> 2) * (AT2_BLOCK_BYTES >> 4) + 2 * (k & 3);
+              tc_mma_bf16_elect(d, da + off, db + off, idesc, k != 0);
+            }
           }
-          tc_commit(&sm.s_full[acc]);
+          tc_commit_elect(&sm.s_full[acc]);
         }
-        if (ok) tc_commit(&sm.b_empty[st]);
+        if (ok) tc_commit_elect(&sm.b_empty[st]);
+        if (++st == n_ring) { st = 0; b_par ^= 1; }
       }
     }
   } else {
-    // ================= the two groups that read accumulators ====================================================
-    const int w = warp >> 2, rr = (warp & 3) * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    At2Row row[2];
-    float2 sum[2];
-    int key[2];
+    // ================= the groups that read accumulators ========================================================
+    // group w reads accumulator w: products w, w + 4, .. of tile w % n_seq; groups with one tile share its columns
+    const int w = warp >> 2, rr = (warp & 3) * 32 + lane, a = w % n_seq, share = AT2_GROUPS / n_seq;
+    const uint32_t col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * AT2_TILE;
+    const bool mine = a < n_a;
+    At2Row row;
+    float2 sum = make_float2(0.f, 0.f);
+    int key = 0;
     const bool missing = PASS == 1 && sm.missing != 0;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int a = n_seq == 4 ? w + 2 * x : (n_seq == 2 ? w : 0);
-      sum[x] = make_float2(0.f, 0.f);
-      if (PASS == 1) {
-        const int t = (a0 + a) * tpt + rr / G;
-        const bool valid = rr < tpt * G && t < R.counted && a < n_a;
-        row[x].m = -INFINITY; row[x].z = 0.f;
-        row[x].pos = R.ctx + t;
-        row[x].hi = valid ? row[x].pos + 1 : 0;
-        row[x].lo = A.window > 0 ? max(0, row[x].pos - A.window + 1) : 0;
-        row[x].slope = GENERAL && A.slopes && valid ? A.slopes[c * G + rr % G] : 0.f;
-      } else {
-        key[x] = (a0 + a) * AT2_TILE + rr;
-      }
+    if (PASS == 1) {
+      const int t = (a0 + a) * tpt + rr / G;
+      const bool valid = rr < tpt * G && t < R.counted && mine;
+      row.m = -INFINITY; row.z = 0.f;
+      row.pos = R.ctx + t;
+      row.hi = valid ? row.pos + 1 : 0;
+      row.lo = A.window > 0 ? max(0, row.pos - A.window + 1) : 0;
+      row.slope = GENERAL && A.slopes && valid ? A.slopes[c * G + rr % G] : 0.f;
+    } else {
+      key = (a0 + a) * AT2_TILE + rr;
     }
     bool ok = true;
-    for (int i = w; i < steps * n_seq; i += 2) {
-      const int s = i / n_seq, a = i - s * n_seq, acc = i & 3;
-      if (a >= n_a) continue;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sm.s_full[acc], (i >> 2) & 1, abort_flag, 5, &g_awtc_status));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t col = lanes + acc * AT2_TILE;
-      const int tile = b0 + s;
-      const bool second = n_seq == 4 && a >= 2;
-      // the second pass: the columns [lo, hi) see this thread's key
-      int lo = 0, hi = 0, dist0 = 0;
-      const float *nm = nullptr, *iv = nullptr;
-      if (PASS == 2) {
-        const int k = second ? key[1] : key[0], tok0 = tile * tpt;
-        lo = max(0, k - R.ctx - tok0) * G;
-        hi = max(0, min(tpt, R.counted - tok0)) * G;
-        if (A.window > 0) hi = (int)max(0L, min((long)hi, ((long)k + A.window - R.ctx - tok0) * G));
-        if (k >= R.total) hi = 0;
-        dist0 = R.ctx + tok0 - k;
-        const size_t at = ((size_t)c * C.tiles + at2_tile0(R, r, tpt) + tile) * AT2_TILE;
-        nm = C.negm + at; iv = C.inv + at;
-      }
-      uint32_t u[2][32];
-      tc_ld_32x32b_x32(col, u[0]);
+    // the second pass: the columns' values of the next tile are on their way while this one's are used, from every warp's own copy
+    const float4* nl_row = PASS == 2 ? reinterpret_cast<const float4*>(C.negl + ((size_t)c * C.tiles + at2_tile0(R, r, tpt) + b0) * AT2_TILE) + lane : nullptr;
+    float4 nl_next = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (PASS == 2 && mine && w / n_seq < steps) nl_next = __ldg(nl_row + (size_t)(w / n_seq) * 32);
+    if (mine)
+      for (int s = w / n_seq, use = 0; s < steps; s += share, ++use) {
+        if (PASS == 2) {
+          sm.negl[warp][use & 1][lane] = nl_next;
+          if (s + share < steps) nl_next = __ldg(nl_row + (size_t)(s + share) * 32);
+          __syncwarp();
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm.s_full[w], use & 1, abort_flag, 5, &g_awtc_status));
+        if (!ok) break;
+        tc_fence_after();
+        const int tile = b0 + s;
+        // the second pass: the columns [lo, hi) see this thread's key
+        int lo = 0, hi = 0, dist0 = 0;
+        if (PASS == 2) {
+          const int tok0 = tile * tpt;
+          lo = max(0, key - R.ctx - tok0) * G;
+          hi = max(0, min(tpt, R.counted - tok0)) * G;
+          if (A.window > 0) hi = (int)max(0L, min((long)hi, ((long)key + A.window - R.ctx - tok0) * G));
+          if (key >= R.total) hi = 0;
+          dist0 = R.ctx + tok0 - key;
+        }
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        at2_wait_ld(u[ch & 1]);
-        if (ch < 3) tc_ld_32x32b_x32(col + 32 * (ch + 1), u[(ch + 1) & 1]);
-        else { tc_fence_before(); mbar_arrive(&sm.s_empty[acc]); }
-        if (PASS == 1) {
-          if (second) at2_row_chunk<GENERAL>(A, R, r, u[ch & 1], tile * AT2_TILE, 32 * ch, row[1], missing);
-          else at2_row_chunk<GENERAL>(A, R, r, u[ch & 1], tile * AT2_TILE, 32 * ch, row[0], missing);
-        } else {
-          if (second) at2_key_chunk<GENERAL>(A, u[ch & 1], 32 * ch, lo, hi, nm, iv, c, G, dist0, sum[1]);
-          else at2_key_chunk<GENERAL>(A, u[ch & 1], 32 * ch, lo, hi, nm, iv, c, G, dist0, sum[0]);
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t u[32];
+          tc_ld_32x32b_x32(col + 32 * ch, u);
+          at2_wait_ld(u);
+          if (ch == 3) { tc_fence_before(); mbar_arrive(&sm.s_empty[w]); }
+          if (PASS == 1) at2_row_chunk<GENERAL>(A, r, u, tile * AT2_TILE, 32 * ch, row, missing);
+          else at2_key_chunk<GENERAL>(A, u, 32 * ch, lo, hi, reinterpret_cast<const float*>(sm.negl[warp][use & 1]), c, G, dist0, sum);
         }
       }
-    }
-    // one A tile: both groups have seen some of its columns
-    if (n_seq == 1) {
-      if (w == 1) sm.meet[rr] = PASS == 1 ? make_float2(row[0].m, row[0].z) : make_float2(sum[0].x + sum[0].y, 0.f);
-      asm volatile("bar.sync 1, 256;\n" ::: "memory");
-      if (w == 0) {
-        const float2 o = sm.meet[rr];
-        if (PASS == 1) {
-          const float m = fmaxf(row[0].m, o.x);
-          if (m != -INFINITY) row[0].z = row[0].z * exp2f(row[0].m - m) + o.y * exp2f(o.x - m);
-          row[0].m = m;
-        } else {
-          sum[0].x += o.x;
-        }
-      }
-    }
-    if (ok && !*abort_flag) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int a = n_seq == 4 ? w + 2 * x : (n_seq == 2 ? w : 0);
-        if (a >= n_a || (x == 1 && n_seq != 4) || (n_seq == 1 && w == 1)) continue;
-        if (PASS == 1) {
-          const int t = (a0 + a) * tpt + rr / G;
-          if (rr < tpt * G && t < R.counted) {
-            float* st = A.stats + (((size_t)(R.row0 + t) * A.Hq + c * G + rr % G) * C.parts + part) * 2;
-            st[0] = row[x].m; st[1] = row[x].z;
-          }
-        } else if (key[x] < R.total) {
-          const int k = key[x];
-          const float total = aw_page(A, r, k) >= 0 ? sum[x].x + sum[x].y : 0.f;
-          if (C.sums) {
-            C.sums[(((size_t)part * A.R + r) * A.Hkv + c) * C.sums_ld + k] = total;
+    float total = sum.x + sum.y;
+    if (n_seq < 4) {
+      // the groups that share a tile put their columns together, in the groups' order
+      sm.meet[w][rr] = PASS == 1 ? make_float2(row.m, row.z) : make_float2(total, 0.f);
+      asm volatile("bar.sync 1, %0;\n" :: "n"(AT2_READERS) : "memory");
+      if (w < n_seq)
+        for (int o = w + n_seq; o < AT2_GROUPS; o += n_seq) {
+          const float2 v = sm.meet[o][rr];
+          if (PASS == 1) {
+            const float m = fmaxf(row.m, v.x);
+            if (m != -INFINITY) row.z = row.z * exp2f(row.m - m) + v.y * exp2f(v.x - m);
+            row.m = m;
           } else {
-            const size_t at = ((size_t)slot * A.Hkv + c) * A.capacity + k;
-            A.out[at] = k < R.ctx ? A.weights[at] + total : total;
-            if (A.positions && k >= R.ctx) A.positions[at] = A.step_positions[R.row0 + k - R.ctx];
+            total += v.x;
           }
+        }
+    }
+    if (ok && !*abort_flag && w < n_seq && mine) {
+      if (PASS == 1) {
+        const int t = (a0 + a) * tpt + rr / G;
+        if (rr < tpt * G && t < R.counted) {
+          float* st = A.stats + (((size_t)(R.row0 + t) * A.Hq + c * G + rr % G) * C.parts + part) * 2;
+          st[0] = row.m; st[1] = row.z;
+        }
+      } else if (key < R.total) {
+        if (aw_page(A, r, key) < 0) total = 0.f;
+        if (C.sums) {
+          C.sums[(((size_t)part * A.R + r) * A.Hkv + c) * C.sums_ld + key] = total;
+        } else {
+          const size_t at = ((size_t)slot * A.Hkv + c) * A.capacity + key;
+          A.out[at] = key < R.ctx ? A.weights[at] + total : total;
+          if (A.positions && key >= R.ctx) A.positions[at] = A.step_positions[R.row0 + key - R.ctx];
         }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (work && warp == 9) {
+  if (work && warp == 4 * AT2_GROUPS + 1) {
     tc_fence_after();
     tc_dealloc(tmem, AT2_COLS);
   }
@@ -401,14 +428,13 @@ attention_weights_merge_kernel(AwArgs A, AwTc C) {
   const AwReq R = aw_req(A, r);
   if ((long)R.n * G <= C.few_rows || tile * C.tpt >= R.counted) return;
   const int t = tile * C.tpt + rr / G;
-  float2 v = make_float2(INFINITY, 0.f);
+  float v = -INFINITY;                              // (a weight of 0)
   if (rr < C.tpt * G && t < R.counted) {
     const int head = c * G + rr % G;
-    v = aw_merge(A.stats + ((size_t)(R.row0 + t) * A.Hq + head) * C.parts * 2, C.parts, A.sinks ? A.sinks + head : nullptr);
+    const float2 mz = aw_merge(A.stats + ((size_t)(R.row0 + t) * A.Hq + head) * C.parts * 2, C.parts, A.sinks ? A.sinks + head : nullptr);
+    if (mz.y > 0.f) v = log2f(mz.y) - mz.x;         // (a row that sees nothing gives nothing)
   }
-  const size_t at = ((size_t)c * C.tiles + at2_tile0(R, r, C.tpt) + tile) * AT2_TILE + rr;
-  C.negm[at] = -v.x;
-  C.inv[at] = v.y;
+  C.negl[((size_t)c * C.tiles + at2_tile0(R, r, C.tpt) + tile) * AT2_TILE + rr] = v;
 }
 
 __global__ void __launch_bounds__(256)
@@ -456,7 +482,7 @@ static cudaError_t at2_launch(dim3 grid, cudaStream_t stream, const CUtensorMap&
   return qe_launch(attention_weights_tc_kernel<PASS, GENERAL>, grid, dim3(AT2_THREADS), smem, stream, q, k, A, C);
 }
 
-// The requests of more than few_rows rows.  stats: [T Hq, parts1, 2] floats; merged: [2, Hkv, T / (128 / G) + R, 128]; sums:
+// The requests of more than few_rows rows.  stats: [T Hq, parts1, 2] floats; merged: [Hkv, T / (128 / G) + R, 128]; sums:
 // [parts2, R, Hkv, max_total] where parts2 > 1.  max_q, max_total: the most tokens of a request and the most places it may hold.
 extern "C" int qe_attention_weights_tc(const void* q, long q_stride, int T, const void* pages, int num_pages, int planes,
                                        const int* block_tables, int max_blocks, const int* cu_q, const int* ctx_lens, const int* slot_ids,
@@ -481,8 +507,7 @@ extern "C" int qe_attention_weights_tc(const void* q, long q_stride, int T, cons
   C.box = 8;
   while (C.box < AT2_TILE && page % (2 * C.box) == 0) C.box *= 2;
   C.tiles = T / C.tpt + R;
-  C.negm = merged;
-  C.inv = merged + (size_t)Hkv * C.tiles * AT2_TILE;
+  C.negl = merged;
   C.sums = parts2 > 1 ? sums : nullptr;
   C.sums_ld = max_total;
   AwArgs A{q, q_stride, T, pages, num_pages, planes, block_tables, max_blocks, cu_q, ctx_lens, slot_ids, counted, step_positions, positions,

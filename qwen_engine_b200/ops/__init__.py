@@ -1799,7 +1799,7 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
         many = [(n, n + c) for n, c in zip(ctx.q_lens_host, ctx.ctx_lens_host) if n * G > few]
         parts1 = attention_weights_tc_parts(sum(-(-n // (tpt * na)) for n, _ in many) * Hkv, -(-max_total // 128))
         parts2 = attention_weights_tc_parts(sum(-(-t // (128 * na)) for _, t in many) * Hkv, -(-max_q // tpt))
-        stats, merged = alloc((T * Hq, parts1, 2), torch.float32), alloc((2, Hkv, T // tpt + R, 128), torch.float32)
+        stats, merged = alloc((T * Hq, parts1, 2), torch.float32), alloc((Hkv, T // tpt + R, 128), torch.float32)
         sums = alloc((parts2, R, Hkv, max_total), torch.float32) if parts2 > 1 else None
         _check(lib().qe_attention_weights_tc(*args, _ptr(stats), parts1, parts2, _ptr(merged), _ptr(sums), max_q, max_total, few, _stream()),
                "accumulate_attention")
