@@ -209,7 +209,7 @@ extern "C" int qe_attention_weights(const void* q, long q_stride, int T, const v
   if (R > 65535 || Hkv > 65535) QE_REFUSE("attention_weights: %d requests, %d kv heads are more than a launch takes", R, Hkv);
   if (parts < 1) QE_REFUSE("attention_weights: %d parts", parts);
   AwArgs A{q, q_stride, T, pages, num_pages, planes, block_tables, max_blocks, cu_q, ctx_lens, slot_ids, counted, step_positions, positions,
-           weights, out, slots, capacity, R, Hq, Hkv, D, page, window, scale, softcap, slopes, sinks, stats, parts};
+           weights, out, slots, capacity, R, Hq, Hkv, D, page, aw_shift(page), window, scale, softcap, slopes, sinks, stats, parts};
   const long row_tiles = ((long)max_q * (Hq / Hkv) + AW_TILE - 1) / AW_TILE, key_tiles = ((long)max_total + AW_TILE - 1) / AW_TILE;
   if (row_tiles * parts > 0x7fffffffL) QE_REFUSE("attention_weights: %d rows are more than a launch takes", max_q);
   const dim3 grid_rows((unsigned)(row_tiles * parts), (unsigned)Hkv, (unsigned)R), grid_keys((unsigned)key_tiles, (unsigned)Hkv, (unsigned)R);

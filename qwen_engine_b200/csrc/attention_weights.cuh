@@ -15,7 +15,7 @@ struct AwArgs {
   const int* step_positions; int* positions;         // positions: null, or where the new tokens' positions are noted
   const float* weights; float* out;                  // [slots, Hkv, capacity]
   int slots; long capacity;
-  int R, Hq, Hkv, D, page, window;
+  int R, Hq, Hkv, D, page, page_shift, window;      // page_shift: log2 of the page, -1 where it is no power of two
   float scale, softcap;
   const float* slopes; const float* sinks;
   float* stats; int parts;                           // [(token * Hq + head), parts, 2]: a part's maximum (of log2) and sum
@@ -44,9 +44,18 @@ __device__ __forceinline__ float aw_score(const AwArgs& A, float x, float slope,
   return x * AW_LOG2E;
 }
 
+__device__ __forceinline__ int aw_block(const AwArgs& A, int key) { return A.page_shift >= 0 ? key >> A.page_shift : key / A.page; }
+__host__ __forceinline__ int aw_shift(int page) {
+  int s = 0;
+  while ((1 << s) < page) ++s;
+  return (1 << s) == page ? s : -1;
+}
+// 2^x by the instruction alone (results below 2^-126 are zero)
+__device__ __forceinline__ float aw_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
+
 // a key's page, or -1: no place of the table, or a place that holds no page
 __device__ __forceinline__ int aw_page(const AwArgs& A, int r, int key) {
-  const int b = key / A.page;
+  const int b = aw_block(A, key);
   if (b >= A.max_blocks) return -1;
   const int p = A.block_tables[(size_t)r * A.max_blocks + b];
   return p < A.num_pages ? p : -1;

@@ -2,8 +2,8 @@
 // request meet each kv head (query tokens x the query heads of its group).  What it computes: attention_weights.cu.
 //
 // The keys are the work: a key's row is 2 D bytes, and all it takes part in are 2 D products per row.  So every key is read
-// once, straight from its page into the registers of the warp that multiplies it (32 keys of up to 128 channels in flight per
-// warp, no shared memory between), and the scores are kept until the rows' sums are known: 4 bytes a row and key.
+// once, straight from its page into the registers of the warp that multiplies it (32 keys of 64 channels while the ones before are multiplied,
+// no shared memory between), and the scores are kept until the rows' sums are known: 4 bytes a row and key.
 //
 // A warp multiplies 32 keys at a time with mma.sync m16n8k16, queries as A, keys as B.  A sum over channels does not care for
 // their order, so a lane's share of B is what it can load in one piece: for the l-th 32 channels lane 4 n + x loads channels 8 x
@@ -25,26 +25,70 @@ __device__ __forceinline__ void af_mma(float (&d)[4], const uint4& a, uint32_t b
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// 16 bytes of a key: read once, so not kept in L1
-__device__ __forceinline__ uint4 af_ld_key(const void* p) {
+// 16 bytes of a key: read once, so not kept in L1, and the first to leave L2 (where the scores stay)
+__device__ __forceinline__ uint64_t af_first_out() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint4 af_ld_key(const void* p, uint64_t policy) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
   return v;
 }
 
 // The scores of the CTA's keys [key0, key1) (key0 a multiple of 32) against the request's rows, in units of log2(e), -inf where
 // a row may not see a key: S[row * ld + key - key0]; and the rows' maxima and sums over those keys into row_max / row_sum (of all MT x 16 rows).
-// MT: tiles of 16 rows; LC: loads of 32 channels in flight per key (2 or 4), `chunks` times.
-template <int MT, int LC>
+// MT: tiles of 16 rows; PLAIN: scores are neither bent nor biased.  A warp goes through its keys 64 channels at a time, the next 64 (of the same
+// 32 keys or of its next ones) on their way while these are multiplied.
+template <int MT, bool PLAIN>
 __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r, int c, int key0, int key1, float* S, size_t ld,
                                           uint4* frags, float (*warp_ml)[MT * 16][2], float* row_max, float* row_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = lane >> 2, x = lane & 3;
   const int G = A.Hq / A.Hkv, rows = R.counted * G;
-  const int chunks = (A.D + 32 * LC - 1) / (32 * LC), steps = chunks * LC * 2;
+  const int chunks = (A.D + 63) / 64, steps = chunks * 4;
+  const uint64_t policy = af_first_out();
+  const bool one_page = A.page % 8 == 0;          // a lane's eight keys lie in one page
+  const size_t page_elems = (size_t)A.planes * A.Hkv * A.page * A.D;
+  // the four keys whose channels this lane loads, of the 32 from j on: 8 (n / 2) + n % 2 + 0, 2, 4, 6; null where there is none
+  auto keys = [&](int j, const __nv_bfloat16* (&kp)[4]) {
+    const int mine = j + 8 * (n >> 1) + (n & 1);
+    const __nv_bfloat16* base = reinterpret_cast<const __nv_bfloat16*>(A.pages) + 8 * x;
+    if (one_page) {
+      const int page = mine < key1 ? aw_page(A, r, mine) : -1;
+      const __nv_bfloat16* p = base + (size_t)max(page, 0) * page_elems + ((size_t)c * A.page + (mine - aw_block(A, mine) * A.page)) * A.D;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) kp[t] = page >= 0 && mine + 2 * t < key1 ? p + 2 * t * A.D : nullptr;
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int key = mine + 2 * t, page = key < key1 ? aw_page(A, r, key) : -1;
+        kp[t] = page >= 0 ? base + (size_t)page * page_elems + ((size_t)c * A.page + (key - aw_block(A, key) * A.page)) * A.D : nullptr;
+      }
+    }
+  };
+  auto fetch = [&](const __nv_bfloat16* const (&kp)[4], int ch, uint4 (&k)[4][2]) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        const int d = 64 * ch + 32 * l;
+        k[t][l] = kp[t] != nullptr && d + 8 * x < A.D ? af_ld_key(kp[t] + d, policy) : make_uint4(0u, 0u, 0u, 0u);
+      }
+  };
+  const int step = AF_WARPS * AF_GROUP;
+  int j0 = key0 + warp * AF_GROUP;
+  const __nv_bfloat16 *kp[4], *kn[4];
+  uint4 cur[4][2], nxt[4][2];
+  if (j0 < key1) {
+    keys(j0, kp);
+    fetch(kp, 0, cur);
+  }
   // the queries as A fragments, in the order of the lanes' channels; rows and channels that do not exist are zero
   for (int i = tid; i < MT * steps * 32; i += AF_THREADS) {
-    const int l = i & 31, step = (i >> 5) % steps, mt = i / (32 * steps);
-    const int d = 32 * (step >> 1) + 8 * (l & 3) + 4 * (step & 1);
+    const int l = i & 31, st = (i >> 5) % steps, mt = i / (32 * steps);
+    const int d = 32 * (st >> 1) + 8 * (l & 3) + 4 * (st & 1);
     uint32_t v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -60,68 +104,51 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
     frags[i] = make_uint4(v[0], v[1], v[2], v[3]);
   }
   __syncthreads();
-  float m[MT][2], z[MT][2], slope[MT][2];
-  int pos[MT][2];
+  float m[MT][2], z[MT][2];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int rho = mt * 16 + 8 * h + n;
-      m[mt][h] = -INFINITY; z[mt][h] = 0.f;
-      pos[mt][h] = rho < rows ? R.ctx + rho / G : -1;
-      slope[mt][h] = A.slopes && rho < rows ? A.slopes[c * G + rho % G] : 0.f;
-    }
-  const bool one_page = A.page % 8 == 0;          // a lane's eight keys lie in one page
-  const size_t page_elems = (size_t)A.planes * A.Hkv * A.page * A.D;
-  for (int j0 = key0 + warp * AF_GROUP; j0 < key1; j0 += AF_WARPS * AF_GROUP) {
-    // the four keys whose channels this lane loads: 8 (n / 2) + n % 2 + 0, 2, 4, 6
-    const int mine = j0 + 8 * (n >> 1) + (n & 1);
-    const __nv_bfloat16* kp[4];
-    if (one_page) {
-      const int page = mine < R.total ? aw_page(A, r, mine) : -1;
-      const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(A.pages) + (size_t)max(page, 0) * page_elems + ((size_t)c * A.page + mine % A.page) * A.D + 8 * x;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) kp[t] = page >= 0 && mine + 2 * t < R.total ? p + 2 * t * A.D : nullptr;
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int key = mine + 2 * t, page = key < R.total ? aw_page(A, r, key) : -1;
-        kp[t] = page >= 0 ? reinterpret_cast<const __nv_bfloat16*>(A.pages) + (size_t)page * page_elems + ((size_t)c * A.page + key % A.page) * A.D + 8 * x : nullptr;
-      }
-    }
+    for (int h = 0; h < 2; ++h) { m[mt][h] = -INFINITY; z[mt][h] = 0.f; }
+  const float sc = A.scale * AW_LOG2E;
+  const int last_pos = R.ctx + max(R.counted, 1) - 1;
+  for (; j0 < key1; j0 += step) {
     float s[MT][4][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int t = 0; t < 4; ++t) s[mt][t][0] = s[mt][t][1] = s[mt][t][2] = s[mt][t][3] = 0.f;
+    const bool more = j0 + step < key1;
+    // which of the warp's 32 keys lie in a page
+    unsigned b[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) b[t] = __ballot_sync(0xffffffffu, kp[t] != nullptr);
+    if (more) keys(j0 + step, kn);
     for (int ch = 0; ch < chunks; ++ch) {
-      uint4 k[4][LC];
+      if (ch + 1 < chunks) fetch(kp, ch + 1, nxt);
+      else if (more) fetch(kn, 0, nxt);
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int l = 0; l < LC; ++l) {
-          const int d = 32 * (ch * LC + l);
-          k[t][l] = kp[t] != nullptr && d + 8 * x < A.D ? af_ld_key(kp[t] + d) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-      for (int l = 0; l < LC; ++l)
+      for (int l = 0; l < 2; ++l)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const uint4* f = frags + ((size_t)mt * steps + 2 * (ch * LC + l)) * 32 + lane;
+          const uint4* f = frags + ((size_t)mt * steps + 4 * ch + 2 * l) * 32 + lane;
           const uint4 a0 = f[0], a1 = f[32];
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            af_mma(s[mt][t], a0, k[t][l].x, k[t][l].y);
-            af_mma(s[mt][t], a1, k[t][l].z, k[t][l].w);
+            af_mma(s[mt][t], a0, cur[t][l].x, cur[t][l].y);
+            af_mma(s[mt][t], a1, cur[t][l].z, cur[t][l].w);
           }
         }
-    }
-    // which of the lane's eight keys of a row, j0 + 8 x .., lie in a page
-    unsigned held = 0u;
-    {
-      unsigned b[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) b[t] = __ballot_sync(0xffffffffu, kp[t] != nullptr);
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int l = 0; l < 2; ++l) cur[t][l] = nxt[t][l];
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) kp[t] = kn[t];
+    // every row sees all 32 keys
+    const bool all = j0 + AF_GROUP <= R.ctx + 1 && (A.window <= 0 || j0 > last_pos - A.window) && (b[0] & b[1] & b[2] & b[3]) == 0xffffffffu;
+    unsigned held = 0u;                             // of the lane's eight keys of a row, j0 + 8 x ..
+    if (!all) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) held |= ((b[e >> 1] >> (4 * (2 * x + (e & 1)))) & 1u) << e;
     }
@@ -129,27 +156,40 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int rho = mt * 16 + 8 * h + n, p = pos[mt][h];
-        float v[8], mx = m[mt][h];
+        if (mt * 16 + 8 * h >= rows) continue;      // (the warp's)
+        const int rho = mt * 16 + 8 * h + n;
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = j0 + 8 * x + e;
-          const bool seen = ((held >> e) & 1u) && key <= p && (A.window <= 0 || key > p - A.window);
-          v[e] = seen ? aw_score(A, s[mt][e >> 1][2 * h + (e & 1)], slope[mt][h], p - key) : -INFINITY;
-          mx = fmaxf(mx, v[e]);
+        for (int e = 0; e < 8; ++e) v[e] = s[mt][e >> 1][2 * h + (e & 1)];
+        if (PLAIN) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= sc;
+        } else {
+          const int p = R.ctx + rho / G;
+          const float slope = A.slopes ? A.slopes[c * G + rho % G] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = aw_score(A, v[e], slope, p - (j0 + 8 * x + e));
+        }
+        if (!all) {
+          const int p = rho < rows ? R.ctx + rho / G : -1;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = j0 + 8 * x + e;
+            if (!(((held >> e) & 1u) && key <= p && (A.window <= 0 || key > p - A.window))) v[e] = -INFINITY;
+          }
         }
         if (rho < rows) {
           float4* dst = reinterpret_cast<float4*>(S + rho * ld + (j0 - key0) + 8 * x);
           dst[0] = make_float4(v[0], v[1], v[2], v[3]);
           dst[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
-        if (mx != -INFINITY) {
-          float sum = z[mt][h] * exp2f(m[mt][h] - mx);
+        const float mx = fmaxf(fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]))), m[mt][h]);
+        const float nb = mx == -INFINITY ? 0.f : -mx;
+        float sum = z[mt][h] * aw_ex2(m[mt][h] + nb);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum += exp2f(v[e] - mx);
-          z[mt][h] = sum;
-          m[mt][h] = mx;
-        }
+        for (int e = 0; e < 8; ++e) sum += aw_ex2(v[e] + nb);
+        z[mt][h] = sum;
+        m[mt][h] = mx;
       }
   }
   // the four lanes of a row, then the warps
@@ -161,7 +201,7 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
       for (int o = 1; o <= 2; o <<= 1) {
         const float om = __shfl_xor_sync(0xffffffffu, m[mt][h], o), oz = __shfl_xor_sync(0xffffffffu, z[mt][h], o);
         const float nm = fmaxf(m[mt][h], om);
-        if (nm != -INFINITY) z[mt][h] = z[mt][h] * exp2f(m[mt][h] - nm) + oz * exp2f(om - nm);
+        if (nm != -INFINITY) z[mt][h] = z[mt][h] * aw_ex2(m[mt][h] - nm) + oz * aw_ex2(om - nm);
         m[mt][h] = nm;
       }
       if (x == 0) { warp_ml[warp][mt * 16 + 8 * h + n][0] = m[mt][h]; warp_ml[warp][mt * 16 + 8 * h + n][1] = z[mt][h]; }
@@ -173,7 +213,7 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
     for (int w = 0; w < AF_WARPS; ++w) mm = fmaxf(mm, warp_ml[w][tid][0]);
     if (mm != -INFINITY)
 #pragma unroll
-      for (int w = 0; w < AF_WARPS; ++w) zz += warp_ml[w][tid][1] * exp2f(warp_ml[w][tid][0] - mm);
+      for (int w = 0; w < AF_WARPS; ++w) zz += warp_ml[w][tid][1] * aw_ex2(warp_ml[w][tid][0] - mm);
     row_max[tid] = mm;
     row_sum[tid] = zz;
   }
@@ -190,7 +230,7 @@ __device__ __forceinline__ bool af_mine(const AwArgs& A, const AwReq& R, int max
 
 // ---- a request's scores in the shared memory of a cluster ----------------------------------------------------------------------
 
-template <int MT, int LC>
+template <int MT, bool PLAIN>
 __global__ void __launch_bounds__(AF_THREADS, 2)
 attention_weights_cluster_kernel(AwArgs A, int max_rows, int part_keys) {
   extern __shared__ __align__(16) unsigned char raw[];
@@ -207,11 +247,11 @@ attention_weights_cluster_kernel(AwArgs A, int max_rows, int part_keys) {
   const int first = af_first(A, R);
   const int per = ((R.total - first + C - 1) / C + AF_GROUP - 1) / AF_GROUP * AF_GROUP;
   const int key0 = min(first + rank * per, R.total), key1 = min(key0 + per, R.total);
-  const int steps = (A.D + 32 * LC - 1) / (32 * LC) * LC * 2;
+  const int steps = (A.D + 63) / 64 * 4;
   uint4* frags = reinterpret_cast<uint4*>(raw);
   float* S = reinterpret_cast<float*>(frags + MT * steps * 32);
   const size_t ld = part_keys + 4;                // (off 32 banks, so that the rows' stores do not meet)
-  af_scores<MT, LC>(A, R, r, c, key0, key1, S, ld, frags, warp_ml, row_max, row_sum);
+  af_scores<MT, PLAIN>(A, R, r, c, key0, key1, S, ld, frags, warp_ml, row_max, row_sum);
   cluster_sync_all();
   if (tid < MT * 16) {
     float m = -INFINITY, z = 0.f;
@@ -229,11 +269,32 @@ attention_weights_cluster_kernel(AwArgs A, int max_rows, int part_keys) {
   }
   cluster_sync_all();                             // (the others' statistics have been read)
   const size_t base = ((size_t)slot * A.Hkv + c) * A.capacity;
-  for (int key = key0 + tid; key < key1; key += AF_THREADS) {
-    float t = 0.f;
-    for (int rho = 0; rho < rows; ++rho) t += exp2f(S[rho * ld + key - key0] - row[rho].x) * row[rho].y;
+  auto finish = [&](int key, float t) {
     A.out[base + key] = key < R.ctx ? A.weights[base + key] + t : t;
     if (A.positions && key >= R.ctx) A.positions[base + key] = A.step_positions[R.row0 + key - R.ctx];
+  };
+  if (key1 - key0 <= AF_THREADS) {                // a key a thread
+    const int key = key0 + tid;
+    if (key < key1) {
+      float t = 0.f;
+#pragma unroll 4
+      for (int rho = 0; rho < rows; ++rho) t = fmaf(aw_ex2(S[rho * ld + tid] - row[rho].x), row[rho].y, t);
+      finish(key, t);
+    }
+  } else {                                        // four
+    for (int key = key0 + 4 * tid; key < key1; key += 4 * AF_THREADS) {
+      float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int rho = 0; rho < rows; ++rho) {
+        const float4 s = *reinterpret_cast<const float4*>(S + rho * ld + (key - key0));
+        const float2 mz = row[rho];
+        t[0] = fmaf(aw_ex2(s.x - mz.x), mz.y, t[0]); t[1] = fmaf(aw_ex2(s.y - mz.x), mz.y, t[1]);
+        t[2] = fmaf(aw_ex2(s.z - mz.x), mz.y, t[2]); t[3] = fmaf(aw_ex2(s.w - mz.x), mz.y, t[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (key + e < key1) finish(key + e, t[e]);
+    }
   }
   if (A.out != A.weights)                         // keys that lie before every row's window
     for (int key = rank * AF_THREADS + tid; key < first; key += C * AF_THREADS) A.out[base + key] = A.weights[base + key];
@@ -242,9 +303,9 @@ attention_weights_cluster_kernel(AwArgs A, int max_rows, int part_keys) {
 // ---- the scores through scratch memory -------------------------------------------------------------------------------------------
 
 // scores: [request, kv head, max_rows, ld]
-template <int MT, int LC>
+template <int MT, bool PLAIN>
 __global__ void __launch_bounds__(AF_THREADS, 2)
-attention_weights_scores_kernel(AwArgs A, int max_rows, float* scores, long ld) {
+attention_weights_scores_kernel(AwArgs A, int max_rows, int least_keys, float* scores, long ld) {
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ float warp_ml[AF_WARPS][MT * 16][2];
   __shared__ float row_max[MT * 16], row_sum[MT * 16];
@@ -255,13 +316,16 @@ attention_weights_scores_kernel(AwArgs A, int max_rows, float* scores, long ld) 
   if (!af_mine(A, R, max_rows)) return;
   const int G = A.Hq / A.Hkv, rows = R.counted * G;
   const int first = af_first(A, R);
-  const int per = ((R.total - first + A.parts - 1) / A.parts + AF_GROUP - 1) / AF_GROUP * AF_GROUP;
+  const int per = (max((R.total - first + A.parts - 1) / A.parts, least_keys) + AF_GROUP - 1) / AF_GROUP * AF_GROUP;
   const int key0 = min(first + part * per, R.total), key1 = min(key0 + per, R.total);
+  float* st = A.stats + ((size_t)(R.row0 + tid / G) * A.Hq + c * G + tid % G) * A.parts * 2 + part * 2;      // of row tid
+  if (key0 == key1) {                             // (a short request has fewer parts)
+    if (tid < rows) { st[0] = -INFINITY; st[1] = 0.f; }
+    return;
+  }
   float* S = scores + (((size_t)r * A.Hkv + c) * max_rows) * ld + (key0 - first);
-  af_scores<MT, LC>(A, R, r, c, key0, key1, S, ld, reinterpret_cast<uint4*>(raw), warp_ml, row_max, row_sum);
+  af_scores<MT, PLAIN>(A, R, r, c, key0, key1, S, ld, reinterpret_cast<uint4*>(raw), warp_ml, row_max, row_sum);
   if (tid < rows) {
-    const int t = tid / G;
-    float* st = A.stats + (((size_t)(R.row0 + t) * A.Hq + c * G + (tid - t * G)) * A.parts + part) * 2;
     st[0] = row_max[tid];
     st[1] = row_sum[tid];
   }
@@ -291,8 +355,8 @@ attention_weights_sum_kernel(AwArgs A, int max_rows, const float* __restrict__ s
     for (int rho = 0; rho < rows; ++rho) {
       const float4 s = __ldcs(reinterpret_cast<const float4*>(S + rho * ld));
       const float2 mz = row[rho];
-      t[0] += exp2f(s.x - mz.x) * mz.y; t[1] += exp2f(s.y - mz.x) * mz.y;
-      t[2] += exp2f(s.z - mz.x) * mz.y; t[3] += exp2f(s.w - mz.x) * mz.y;
+      t[0] = fmaf(aw_ex2(s.x - mz.x), mz.y, t[0]); t[1] = fmaf(aw_ex2(s.y - mz.x), mz.y, t[1]);
+      t[2] = fmaf(aw_ex2(s.z - mz.x), mz.y, t[2]); t[3] = fmaf(aw_ex2(s.w - mz.x), mz.y, t[3]);
     }
   }
   const size_t base = ((size_t)slot * A.Hkv + c) * A.capacity;
@@ -307,8 +371,7 @@ attention_weights_sum_kernel(AwArgs A, int max_rows, const float* __restrict__ s
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 
-static int af_lc(int D) { return D <= 64 ? 2 : 4; }
-static size_t af_frag_bytes(int mt, int D) { const int lc = af_lc(D); return (size_t)mt * ((D + 32 * lc - 1) / (32 * lc)) * lc * 2 * 512; }
+static size_t af_frag_bytes(int mt, int D) { return (size_t)mt * ((D + 63) / 64) * 4 * 512; }
 
 // Shared memory of a CTA of the cluster form for parts of `part_keys` keys; 0 where the kernels do not take the sizes.
 extern "C" long qe_attention_weights_few_smem(int max_rows, int D, int part_keys) {
@@ -317,38 +380,38 @@ extern "C" long qe_attention_weights_few_smem(int max_rows, int D, int part_keys
   return (long)af_frag_bytes(mt, D) + (long)max_rows * (part_keys + 4) * 4;
 }
 
-template <int MT, int LC>
+template <int MT, bool PLAIN>
 static cudaError_t af_launch(const AwArgs& A, int max_rows, int ctas, int part_keys, size_t smem, float* scores, long ld, int max_total, cudaStream_t stream) {
   if (ctas > 0) {
     if (smem > 48 * 1024) {
       static bool configured = false;
       if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attention_weights_cluster_kernel<MT, LC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        cudaError_t e = cudaFuncSetAttribute(attention_weights_cluster_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
         if (e != cudaSuccess) return e;
         configured = true;
       }
     }
-    return qe_launch_cluster(attention_weights_cluster_kernel<MT, LC>, dim3((unsigned)ctas, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), smem, stream,
+    return qe_launch_cluster(attention_weights_cluster_kernel<MT, PLAIN>, dim3((unsigned)ctas, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), smem, stream,
                              (unsigned)ctas, A, max_rows, part_keys);
   }
   const size_t frag = af_frag_bytes(MT, A.D);
   if (frag > 48 * 1024) {
     static bool configured = false;
     if (!configured) {
-      cudaError_t e = cudaFuncSetAttribute(attention_weights_scores_kernel<MT, LC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+      cudaError_t e = cudaFuncSetAttribute(attention_weights_scores_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
       if (e != cudaSuccess) return e;
       configured = true;
     }
   }
-  cudaError_t e = qe_launch(attention_weights_scores_kernel<MT, LC>, dim3((unsigned)A.parts, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), frag, stream,
-                            A, max_rows, scores, ld);
+  cudaError_t e = qe_launch(attention_weights_scores_kernel<MT, PLAIN>, dim3((unsigned)A.parts, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), frag, stream,
+                            A, max_rows, part_keys, scores, ld);
   if (e != cudaSuccess) return e;
   return qe_launch(attention_weights_sum_kernel, dim3((unsigned)((max_total + AF_THREADS * 4 - 1) / (AF_THREADS * 4)), (unsigned)A.Hkv, (unsigned)A.R),
                    dim3(AF_THREADS), 0, stream, A, max_rows, (const float*)scores, ld);
 }
 
 // The requests of at most `max_rows` rows (a query token x a query head of a kv head's group), 32 at most.  ctas > 0: clusters of so many
-// CTAs (1, 2, 4, 8) hold the scores, part_keys keys a CTA at most (a multiple of 32; span <= ctas part_keys); 0: `scores`, scratch
+// CTAs (1, 2, 4, 8) hold the scores, part_keys keys a CTA at most (a multiple of 32; span <= ctas part_keys); 0: parts of at least part_keys, and `scores`, scratch
 // memory of [R, Hkv, max_rows, ld] floats with ld a multiple of 4 and at least span + 32, does.  span: the most keys that a request's rows
 // see between them, from a multiple of 32 on (max_total without a window).
 extern "C" int qe_attention_weights_few(const void* q, long q_stride, int T, const void* pages, int num_pages, int planes,
@@ -367,11 +430,11 @@ extern "C" int qe_attention_weights_few(const void* q, long q_stride, int T, con
   if (ctas == 0 && (scores == nullptr || stats == nullptr || parts < 1 || ld % 4 || ld < span + AF_GROUP))
     QE_REFUSE("attention_weights: scratch memory for %d keys is needed", span);
   AwArgs A{q, q_stride, T, pages, num_pages, planes, block_tables, max_blocks, cu_q, ctx_lens, slot_ids, counted, step_positions, positions,
-           weights, out, slots, capacity, R, Hq, Hkv, D, page, window, scale, softcap, slopes, sinks, stats, parts};
-  const bool two = max_rows > 16, wide = af_lc(D) == 4;
+           weights, out, slots, capacity, R, Hq, Hkv, D, page, aw_shift(page), window, scale, softcap, slopes, sinks, stats, parts};
+  const bool plain = softcap <= 0.f && slopes == nullptr;
   cudaError_t e;
-  if (two) e = wide ? af_launch<2, 4>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream) : af_launch<2, 2>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream);
-  else e = wide ? af_launch<1, 4>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream) : af_launch<1, 2>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream);
+  if (max_rows > 16) e = plain ? af_launch<2, true>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream) : af_launch<2, false>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream);
+  else e = plain ? af_launch<1, true>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream) : af_launch<1, false>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream);
   if (e != cudaSuccess) { qe_set_error("attention_weights: launch failed: %s", cudaGetErrorString(e)); (void)cudaGetLastError(); return 2; }
   QE_CHECK_LAUNCH("attention_weights");
   return 0;

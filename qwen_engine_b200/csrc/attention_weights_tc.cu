@@ -511,7 +511,7 @@ extern "C" int qe_attention_weights_tc(const void* q, long q_stride, int T, cons
   C.sums = parts2 > 1 ? sums : nullptr;
   C.sums_ld = max_total;
   AwArgs A{q, q_stride, T, pages, num_pages, planes, block_tables, max_blocks, cu_q, ctx_lens, slot_ids, counted, step_positions, positions,
-           weights, out, slots, capacity, R, Hq, Hkv, D, page, window, scale, softcap, slopes, sinks, stats, parts1};
+           weights, out, slots, capacity, R, Hq, Hkv, D, page, aw_shift(page), window, scale, softcap, slopes, sinks, stats, parts1};
   CUtensorMap map_q, map_k;
   {
     const uint64_t dims[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)T};

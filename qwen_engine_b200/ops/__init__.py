@@ -1696,19 +1696,20 @@ def _attention_weights_parts(row_tiles: int, heads: int, requests: int, max_tota
 
 
 ATTENTION_WEIGHTS_FEW_ROWS = 32               # rows of a request (a query token x a query head of a kv head's group) up to which the kernel of few rows serves
-ATTENTION_WEIGHTS_CLUSTER_SMEM = 110 * 1024   # bytes of scores up to which a request's rows and keys are shared by a cluster: two CTAs an SM
+ATTENTION_WEIGHTS_CLUSTER_MAX_CTAS = 148      # clusters of 8 share a request's keys where they are so few CTAs at most ...
+ATTENTION_WEIGHTS_CLUSTER_MAX_KEYS = 4096     # ... and so few keys: one launch, 6.3 us for 1 request of 1 024 keys (16 / 8 heads; 8.3 through scratch memory);
+                                              # more of either is faster through scratch memory, whose CTAs need not start together (8 requests of 1 088 keys
+                                              # 12.5 against 15.9 us, 32 x 5 rows of up to 8 200 keys, 32 / 8 heads, 76 against 118, 1 request of 32 000 keys 23 against 36)
+ATTENTION_WEIGHTS_CLUSTER_SMEM = 110 * 1024   # bytes of shared memory of such a CTA at most
 
 
 def attention_weights_cluster(rows: int, heads: int, head_dim: int, requests: int, span: int) -> tuple[int, int]:
-    """(CTAs of a cluster, keys a CTA) for the gathered weights of a few rows, (0, 0) where scratch memory holds the scores: as many
-    of 1, 2, 4, 8 CTAs as give every SM two."""
-    ctas = 1
-    while ctas < 8 and (requests * heads * ctas < FLASH_TARGET_CTAS or _cluster_smem(rows, head_dim, -(-span // ctas)) > ATTENTION_WEIGHTS_CLUSTER_SMEM):
-        ctas *= 2
-    part = -(-span // (32 * ctas)) * 32
-    if _cluster_smem(rows, head_dim, part) > ATTENTION_WEIGHTS_CLUSTER_SMEM:
-        return 0, 0
-    return ctas, part
+    """(CTAs of a cluster, keys a CTA) for the gathered weights of a few rows; (0, least keys of a part) where scratch memory
+    holds the scores: about 256 CTAs, of 512 to 2 048 keys each."""
+    part = -(-span // 256) * 32
+    if requests * heads * 8 <= ATTENTION_WEIGHTS_CLUSTER_MAX_CTAS and span <= ATTENTION_WEIGHTS_CLUSTER_MAX_KEYS and _cluster_smem(rows, head_dim, part) <= ATTENTION_WEIGHTS_CLUSTER_SMEM:
+        return 8, part
+    return 0, min(2048, max(512, -(-requests * heads * span // (256 * 32)) * 32))
 
 
 ATTENTION_WEIGHTS_TC = True                   # more rows in bfloat16: the kernels on the tensor cores (False: the general kernels serve them)
@@ -1721,8 +1722,7 @@ def attention_weights_tc_parts(units: int, tiles: int) -> int:
 
 def _cluster_smem(rows: int, head_dim: int, part: int) -> int:
     """Shared memory of a CTA of that kernel: the queries as fragments, and its keys' scores."""
-    lc = 2 if head_dim <= 64 else 4
-    return (2 if rows > 16 else 1) * -(-head_dim // (32 * lc)) * lc * 1024 + rows * (part + 4) * 4
+    return (2 if rows > 16 else 1) * -(-head_dim // 64) * 2048 + rows * (part + 4) * 4
 
 
 def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables: torch.Tensor, ctx, weights: torch.Tensor,
@@ -1785,7 +1785,7 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
         ctas, part_keys = attention_weights_cluster(few, Hkv, D, R, span)
         scores, ld, parts, stats = None, 0, 1, None
         if ctas == 0:
-            parts = _attention_weights_parts(1, Hkv, R, span)
+            parts = min(-(-span // part_keys), ATTENTION_WEIGHTS_MAX_PARTS)
             ld = -(-(span + 32) // 32) * 32
             scores, stats = alloc((R, Hkv, few, ld), torch.float32), alloc((T * Hq, parts, 2), torch.float32)
         _check(lib().qe_attention_weights_few(*args, _ptr(stats), parts, few, max_total, span, ctas, part_keys, _ptr(scores), ctypes.c_long(ld), _stream()),

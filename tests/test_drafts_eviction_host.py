@@ -105,3 +105,20 @@ def test_parts_of_rows():
     assert ops._attention_weights_parts(64, 8, 1, 4096) == 1
     assert ops._attention_weights_parts(1, 8, 1, 4096) == 16 and ops._attention_weights_parts(1, 8, 1, 131072) == 37
     assert ops._attention_weights_parts(1, 1, 1, 1 << 20) == ops.ATTENTION_WEIGHTS_MAX_PARTS and ops._attention_weights_parts(1, 1, 1, 1) == 1
+
+
+def test_where_a_few_rows_scores_go():
+    """Short contexts of few requests: a cluster's shared memory, parts that hold every key; else scratch memory, parts of 512 to 2 048 keys."""
+    for rows in (1, 2, 16, 17, 32):
+        for span in (1, 31, 32, 33, 1000, 4096, 4097, 100000):
+            for requests in (1, 2, 3, 64):
+                ctas, part = ops.attention_weights_cluster(rows, 8, 128, requests, span)
+                assert part % 32 == 0
+                if ctas:
+                    assert ctas == 8 and ctas * part >= span and requests <= 2 and span <= 4096
+                else:
+                    assert 512 <= part <= 2048 and (requests > 2 or span > 4096 or ops._cluster_smem(rows, 128, -(-span // 256) * 32) > 110 * 1024)
+    for units in (1, 7, 64, 1000):
+        for tiles in (1, 3, 4, 100):
+            parts = ops.attention_weights_tc_parts(units, tiles)
+            assert 1 <= parts <= max(1, -(-tiles // 4)) and (parts == 1 or (parts - 1) * units < 4 * 148)
