@@ -7,9 +7,14 @@
 // which does not look at the order of its keys, reads `keep` entries as one run of places.
 //
 // Selecting.  The entries' ranks are keys: an order-preserving integer of the weight, the largest integer for those that stay
-// in any case.  The keep-th largest key is found digit by digit (8 bits a pass) from histograms; a cluster of CTAs shares a
-// head's entries where there are many, its histograms and counts meeting in distributed shared memory.  Then everybody's
-// place in the lists of movers and of free places follows from counts in the order of the entries.
+// in any case.  They are formed once, into shared memory; the keep-th largest is found digit by digit (8 bits a pass) from
+// histograms; a cluster of CTAs shares a head's entries where there are many, its histograms and counts meeting in
+// distributed shared memory (two histograms in turn, so that a pass is one meeting).  The last pass's histogram also says how many
+// entries of every CTA are at the threshold, of which the lowest places stay.  Everybody's place in the lists of movers and of
+// free places then follows from ballots in the order of the entries, a warp a run of them.
+//
+// What bounds it: moving bulk, the copies (an entry's planes are 16 bytes a lane, four entries of a warp on their way at a time); a
+// step's eviction of an entry, the chain of meetings.
 #include "common.cuh"
 #include <math.h>
 
@@ -17,6 +22,8 @@
 #define EV_WARPS (EV_THREADS / 32)
 #define EV_MAX_CTAS 8
 #define EV_PER_CTA 4096          // entries of a head from which one more CTA joins its cluster
+#define EV_MAX_SMEM (200 * 1024)
+#define EV_MOVES_INSIDE 64       // moves of a head, at most, that the selecting kernel makes itself
 
 struct EvArgs {
   const int* block_tables; int max_blocks; int num_pages;
@@ -24,6 +31,7 @@ struct EvArgs {
   const float* weights; const int* positions; float* weights_out; int* positions_out;
   long head_stride;              // capacity: entries between a (layer, slot, head)'s row and the next
   int slots, Hkv, R, capacity, keep, first, recent;
+  char* cache; int planes, page, row_bytes;
   int* moves;                    // [layer, request, head]: 1 + 2 keep ints: how many, the places they come from, the places they go to
 };
 
@@ -37,37 +45,52 @@ __device__ __forceinline__ int ev_ld_remote(const int* local, int cta) {
   asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(cluster_map_shared(local, cta)) : "memory");
   return v;
 }
-__device__ __forceinline__ int ev_block_sum(int v, int* s) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int t = 0;
-  for (int w = 0; w < EV_WARPS; ++w) t += s[w];
-  return t;
-}
-// the sum over the threads before this one, and over all (`total`)
-__device__ __forceinline__ int ev_block_before(bool flag, int* s, int& total) {
-  const unsigned b = __ballot_sync(0xffffffffu, flag);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
-  if (lane == 0) s[warp] = __popc(b);
-  __syncthreads();
-  int before = __popc(b & ((1u << lane) - 1u));
-  total = 0;
-  for (int w = 0; w < EV_WARPS; ++w) {
-    if (w < warp) before += s[w];
-    total += s[w];
+
+// The keys and values of moves first, first + step, .. below n: a warp an entry, V what one lane moves at a time, four entries on their way.
+template <typename V>
+__device__ __forceinline__ void ev_move(const EvArgs& A, int layer, int r, int h, const int* moves, int n, int first, int step) {
+  const int* table = A.block_tables + (size_t)r * A.max_blocks;
+  const size_t plane_bytes = (size_t)A.Hkv * A.page * A.row_bytes;
+  char* base = A.cache + (size_t)layer * A.num_pages * A.planes * plane_bytes + (size_t)h * A.page * A.row_bytes;
+  const int lane = threadIdx.x & 31, vecs = A.row_bytes / (int)sizeof(V), all = A.planes * vecs;
+  auto place = [&](int at) -> char* {             // null where no page is held
+    const int b = at / A.page, p = table[b];
+    return p >= 0 && p < A.num_pages ? base + (size_t)p * A.planes * plane_bytes + (size_t)(at - b * A.page) * A.row_bytes : nullptr;
+  };
+  for (int i = first; i < n; i += 4 * step) {
+    const V* src[4];
+    V* dst[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      src[e] = nullptr; dst[e] = nullptr;
+      if (i + e * step < n) {
+        char* f = place(__ldcg(moves + 1 + i + e * step));
+        char* t = place(__ldcg(moves + 1 + A.keep + i + e * step));
+        if (f && t) { src[e] = reinterpret_cast<const V*>(f); dst[e] = reinterpret_cast<V*>(t); }
+      }
+    }
+    for (int v = lane; v < all; v += 32) {
+      const int pl = v / vecs;
+      const size_t o = (pl * plane_bytes) / sizeof(V) + (v - pl * vecs);
+      V x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (src[e]) x[e] = src[e][o];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (src[e]) dst[e][o] = x[e];
+    }
   }
-  return before;
 }
 
+// held: the keys lie in shared memory (else they are formed again wherever they are looked at).  MOVES: 0 where another kernel moves the
+// entries, else the bytes that a lane moves at a time.
+template <int MOVES>
 __global__ void __launch_bounds__(EV_THREADS)
-evict_select_kernel(EvArgs A) {
-  __shared__ int hist[256];
-  __shared__ int s_red[EV_WARPS];
-  __shared__ int x[4];                          // read by the other CTAs of the cluster
-  __shared__ int digit_s, above_s, warp_tot[8];
+evict_select_kernel(EvArgs A, int held) {
+  extern __shared__ unsigned keys[];
+  __shared__ int hist[2][256];
+  __shared__ int s_max[EV_WARPS], s_ties[EV_WARPS], s_holes[EV_WARPS], s_movers[EV_WARPS], warp_tot[8];
+  __shared__ int x[3];                          // read by the other CTAs of the cluster: latest position, free places, movers
+  __shared__ int digit_s, above_s;
   pdl_launch_dependents();
   pdl_wait();
   const int C = (int)cluster_num_ctas(), rank = (int)cluster_cta_rank();
@@ -95,37 +118,63 @@ evict_select_kernel(EvArgs A) {
   }
   // the latest position
   int latest = -0x7fffffff;
-  for (int j = e0 + tid; j < e1; j += EV_THREADS) latest = max(latest, P[j]);
-  latest = __reduce_max_sync(0xffffffffu, latest);
-  if (lane == 0) s_red[warp] = latest;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < EV_WARPS; ++w) latest = max(latest, s_red[w]);
-    x[0] = latest;
+  for (int j = e0 + tid; j < e1; j += 4 * EV_THREADS) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i * EV_THREADS < e1) latest = max(latest, P[j + i * EV_THREADS]);
   }
-  cluster_sync_all();
-  latest = ev_ld_remote(&x[0], 0);
-  for (int o = 1; o < C; ++o) latest = max(latest, ev_ld_remote(&x[0], o));
-  const int recent_from = latest - A.recent;
-  auto key_of = [&](int j) {
-    const int p = P[j];
-    return p < A.first || p > recent_from ? 0xffffffffu : ev_key(W[j]);
-  };
-  // the keep-th largest key
-  unsigned thr = 0u;
-  int left = keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += EV_THREADS) hist[i] = 0;
-    __syncthreads();
-    const unsigned mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int j = e0 + tid; j < e1; j += EV_THREADS) {
-      const unsigned key = key_of(j);
-      if ((key & mask) == (thr & mask)) atomicAdd(&hist[(key >> shift) & 255u], 1);
-    }
+  latest = __reduce_max_sync(0xffffffffu, latest);
+  if (lane == 0) s_max[warp] = latest;
+  if (tid < 256) { hist[0][tid] = 0; hist[1][tid] = 0; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < EV_WARPS; ++w) latest = max(latest, s_max[w]);
+  if (C > 1) {
+    if (tid == 0) x[0] = latest;
     cluster_sync_all();
-    int c = 0;
-    if (tid < 256)
-      for (int o = 0; o < C; ++o) c += ev_ld_remote(&hist[255 - tid], o);
+#pragma unroll
+    for (int o = 0; o < EV_MAX_CTAS; ++o) if (o < C) latest = max(latest, ev_ld_remote(&x[0], o));
+  }
+  const int recent_from = latest - A.recent;
+  auto key_of = [&](int p, float w) { return p < A.first || p > recent_from ? 0xffffffffu : ev_key(w); };
+  auto key_at = [&](int j) { return held ? keys[j - e0] : key_of(P[j], W[j]); };
+  // the keep-th largest key; the first pass forms the keys
+  unsigned thr = 0u;
+  int left = keep, ties_before = 0;
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    int* const hs = hist[pass & 1];
+    if (pass == 0) {
+      for (int j = e0 + tid; j < e1; j += 4 * EV_THREADS) {
+        int p[4];
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i * EV_THREADS < e1) { p[i] = P[j + i * EV_THREADS]; w[i] = W[j + i * EV_THREADS]; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i * EV_THREADS < e1) {
+            const unsigned key = key_of(p[i], w[i]);
+            if (held) keys[j + i * EV_THREADS - e0] = key;
+            atomicAdd(&hs[key >> 24], 1);
+          }
+      }
+    } else {
+      const unsigned mask = 0xffffffffu << (shift + 8);
+      for (int j = e0 + tid; j < e1; j += EV_THREADS) {
+        const unsigned key = key_at(j);
+        if ((key & mask) == thr) atomicAdd(&hs[(key >> shift) & 255u], 1);
+      }
+    }
+    cluster_sync_all();                           // (of one CTA: its threads)
+    int c = 0, mine[EV_MAX_CTAS];
+    if (tid < 256) {
+#pragma unroll
+      for (int o = 0; o < EV_MAX_CTAS; ++o) mine[o] = o < C ? ev_ld_remote(&hs[255 - tid], o) : 0;
+#pragma unroll
+      for (int o = 0; o < EV_MAX_CTAS; ++o) c += mine[o];
+      hist[(pass & 1) ^ 1][tid] = 0;              // everybody has read it: they are past this pass's meeting
+    }
     int run = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -136,91 +185,111 @@ evict_select_kernel(EvArgs A) {
     __syncthreads();
     if (tid < 256) {
       for (int w = 0; w < warp; ++w) run += warp_tot[w];
-      if (run >= left && run - c < left) { digit_s = 255 - tid; above_s = run - c; }
+      if (run >= left && run - c < left) {
+        digit_s = 255 - tid;
+        above_s = run - c;
+        int before = 0;                           // (last pass: entries at the threshold in the CTAs before this one)
+#pragma unroll
+        for (int o = 0; o < EV_MAX_CTAS; ++o) if (o < rank) before += mine[o];
+        x[0] = before;                            // (the others have read their copies of it long ago)
+      }
     }
     __syncthreads();
     thr |= (unsigned)digit_s << shift;
     left -= above_s;
-    cluster_sync_all();
+    ties_before = x[0];
   }
-  // `left` of the entries at the threshold stay, the lowest places
-  int ties = 0;
-  for (int j = e0 + tid; j < e1; j += EV_THREADS) ties += key_of(j) == thr;
-  ties = ev_block_sum(ties, s_red);
-  if (tid == 0) x[1] = ties;
-  cluster_sync_all();
-  int ties_before = 0;
-  for (int o = 0; o < rank; ++o) ties_before += ev_ld_remote(&x[1], o);
-  // twice over the entries in their order: count movers and free places, then list them
-  int holes = 0, movers = 0;                    // of the CTAs before this one (second time)
-  for (int pass = 0; pass < 2; ++pass) {
-    int t_run = ties_before, h_run = holes, m_run = movers;
-    for (int b = e0; b < e1; b += EV_THREADS) {
-      const int j = b + tid;
-      const bool in = j < e1;
-      const unsigned key = in ? key_of(j) : 0u;
-      int tot;
-      const int t_before = t_run + ev_block_before(in && key == thr, s_red, tot);
-      t_run += tot;
-      const bool stays = in && (key > thr || (key == thr && t_before < left));
-      const bool hole = in && !stays && j < keep, mover = stays && j >= keep;
-      const int h_at = h_run + ev_block_before(hole, s_red, tot);
-      h_run += tot;
-      const int m_at = m_run + ev_block_before(mover, s_red, tot);
-      m_run += tot;
-      if (pass == 1) {
-        if (mover) moves[1 + m_at] = j;
-        if (hole) moves[1 + keep + h_at] = j;
-        if (stays && j < keep) {
-          if (Wo != W) Wo[j] = W[j];
-          if (Po != P) Po[j] = P[j];
-        }
-      }
+  // `left` of the entries at the threshold stay, the lowest places.  A warp has a run of entries: its ties, then its free places and movers, then the lists.
+  const int run_len = (per / 32 + EV_WARPS - 1) / EV_WARPS * 32;
+  const int j0 = min(e1, e0 + warp * run_len), j1 = min(e1, j0 + run_len);
+  int n = 0;
+  for (int j = j0; j < j1; j += 32) n += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && key_at(j + lane) == thr));
+  if (lane == 0) s_ties[warp] = n;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) ties_before += s_ties[w];
+  const unsigned below = (1u << lane) - 1u;
+  // what the 32 entries from j on do: which stay, with `ties` the ties before them
+  auto stay = [&](int j, int& ties) {
+    const unsigned key = j + lane < j1 ? key_at(j + lane) : 0u;
+    const unsigned same = __ballot_sync(0xffffffffu, j + lane < j1 && key == thr);
+    const bool s = j + lane < j1 && (key > thr || (key == thr && ties + __popc(same & below) < left));
+    ties += __popc(same);
+    return s;
+  };
+  int holes = 0, movers = 0, ties = ties_before;
+  for (int j = j0; j < j1; j += 32) {
+    const bool s = stay(j, ties);
+    holes += __popc(__ballot_sync(0xffffffffu, !s && j + lane < min(j1, keep)));
+    movers += __popc(__ballot_sync(0xffffffffu, s && j + lane >= keep));
+  }
+  if (lane == 0) { s_holes[warp] = holes; s_movers[warp] = movers; }
+  __syncthreads();
+  holes = movers = 0;
+  int all_movers = 0, cta_holes = 0;
+#pragma unroll
+  for (int w = 0; w < EV_WARPS; ++w) {
+    if (w < warp) { holes += s_holes[w]; movers += s_movers[w]; }
+    cta_holes += s_holes[w];
+    all_movers += s_movers[w];
+  }
+  if (C > 1) {
+    if (tid == 0) { x[1] = cta_holes; x[2] = all_movers; }
+    cluster_sync_all();
+    int hs[EV_MAX_CTAS], ms[EV_MAX_CTAS];
+#pragma unroll
+    for (int o = 0; o < EV_MAX_CTAS; ++o) { hs[o] = o < C ? ev_ld_remote(&x[1], o) : 0; ms[o] = o < C ? ev_ld_remote(&x[2], o) : 0; }
+    all_movers = 0;
+#pragma unroll
+    for (int o = 0; o < EV_MAX_CTAS; ++o) {
+      if (o < rank) { holes += hs[o]; movers += ms[o]; }
+      all_movers += ms[o];
     }
-    if (pass == 0) {
-      if (tid == 0) { x[2] = h_run; x[3] = m_run; }
-      cluster_sync_all();
-      for (int o = 0; o < rank; ++o) { holes += ev_ld_remote(&x[2], o); movers += ev_ld_remote(&x[3], o); }
-      int all = 0;
-      for (int o = 0; o < C; ++o) all += ev_ld_remote(&x[3], o);
-      if (rank == 0 && tid == 0) moves[0] = all;
+  }
+  if (rank == 0 && tid == 0) moves[0] = all_movers;
+  ties = ties_before;
+  for (int j = j0; j < j1; j += 32) {
+    const bool s = stay(j, ties), in = j + lane < j1;
+    const unsigned hb = __ballot_sync(0xffffffffu, !s && j + lane < min(j1, keep)), mb = __ballot_sync(0xffffffffu, s && j + lane >= keep);
+    if ((hb >> lane) & 1u) moves[1 + keep + holes + __popc(hb & below)] = j + lane;
+    if ((mb >> lane) & 1u) moves[1 + movers + __popc(mb & below)] = j + lane;
+    holes += __popc(hb);
+    movers += __popc(mb);
+    if (in && s && j + lane < keep) {
+      if (Wo != W) Wo[j + lane] = W[j + lane];
+      if (Po != P) Po[j + lane] = P[j + lane];
     }
   }
   __threadfence();
-  cluster_sync_all();                           // both lists are whole
-  const int n = *reinterpret_cast<volatile int*>(moves);
-  for (int i = rank * EV_THREADS + tid; i < n; i += C * EV_THREADS) {
+  cluster_sync_all();                           // both lists are whole, and nobody's shared memory is read any more
+  for (int i = rank * EV_THREADS + tid; i < all_movers; i += C * EV_THREADS) {
     const int from = __ldcg(moves + 1 + i), to = __ldcg(moves + 1 + keep + i);
     Wo[to] = W[from];
     Po[to] = P[from];
   }
+  if (MOVES == 16) ev_move<uint4>(A, layer, r, h, moves, all_movers, rank * EV_WARPS + warp, C * EV_WARPS);
+  if (MOVES == 4) ev_move<uint32_t>(A, layer, r, h, moves, all_movers, rank * EV_WARPS + warp, C * EV_WARPS);
+  if (MOVES == 2) ev_move<uint16_t>(A, layer, r, h, moves, all_movers, rank * EV_WARPS + warp, C * EV_WARPS);
 }
 
-// The listed entries' keys and values, a warp an entry; V is what one lane moves at a time.
 template <typename V>
 __global__ void __launch_bounds__(256)
-evict_move_kernel(EvArgs A, char* cache, int planes, int page_size, int row_bytes) {
+evict_move_kernel(EvArgs A) {
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.y / A.Hkv, h = blockIdx.y - r * A.Hkv, layer = blockIdx.z;
   const int* moves = A.moves + (((size_t)layer * A.R + r) * A.Hkv + h) * (size_t)(1 + 2 * A.keep);
-  const int n = moves[0];
-  const int* table = A.block_tables + (size_t)r * A.max_blocks;
-  const size_t plane_bytes = (size_t)A.Hkv * page_size * row_bytes;
-  char* base = cache + (size_t)layer * A.num_pages * planes * plane_bytes;
-  const int lane = threadIdx.x & 31, vecs = row_bytes / (int)sizeof(V);
-  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
-    const int from = moves[1 + i], to = moves[1 + A.keep + i];
-    const int fb = from / page_size, tb = to / page_size;
-    const int fp = table[fb], tp = table[tb];
-    if (fp < 0 || tp < 0 || fp >= A.num_pages || tp >= A.num_pages) continue;     // no page held there
-    const char* src = base + (size_t)fp * planes * plane_bytes + ((size_t)h * page_size + (from - fb * page_size)) * row_bytes;
-    char* dst = base + (size_t)tp * planes * plane_bytes + ((size_t)h * page_size + (to - tb * page_size)) * row_bytes;
-    for (int v = lane; v < planes * vecs; v += 32) {
-      const int pl = v / vecs, o = v - pl * vecs;
-      reinterpret_cast<V*>(dst + pl * plane_bytes)[o] = reinterpret_cast<const V*>(src + pl * plane_bytes)[o];
-    }
+  ev_move<V>(A, layer, r, h, moves, moves[0], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
+}
+
+template <int MOVES>
+static cudaError_t ev_select(dim3 grid, size_t smem, cudaStream_t stream, const EvArgs& args, int held) {
+  static bool configured = false;
+  if (smem > 48 * 1024 && !configured) {
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<MOVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_SMEM);
+    if (e != cudaSuccess) return e;
+    configured = true;
   }
+  return qe_launch_cluster(evict_select_kernel<MOVES>, grid, dim3(EV_THREADS), smem, stream, grid.x, args, held);
 }
 
 extern "C" int qe_evict_tokens(void* cache, int layers, int num_pages, int planes, int Hkv, int page_size, int row_bytes,
@@ -231,21 +300,30 @@ extern "C" int qe_evict_tokens(void* cache, int layers, int num_pages, int plane
   if (keep < 1 || first < 0 || recent < 0) QE_REFUSE("evict_tokens: a budget of %d with %d first and %d recent entries", keep, first, recent);
   if ((long)R * Hkv > 65535 || layers > 65535) QE_REFUSE("evict_tokens: %d requests of %d heads, %d layers are more than a launch takes", R, Hkv, layers);
   EvArgs args{block_tables, max_blocks, num_pages, slot_ids, lens, weights, positions, weights_out, positions_out, head_stride,
-              slots, Hkv, R, capacity, keep, first, recent, moves};
+              slots, Hkv, R, capacity, keep, first, recent, (char*)cache, planes, page_size, row_bytes, moves};
   unsigned ctas = 1;
   while (ctas < EV_MAX_CTAS && (long)ctas * EV_PER_CTA < capacity) ctas *= 2;
-  qe_launch_cluster(evict_select_kernel, dim3(ctas, (unsigned)(R * Hkv), (unsigned)layers), dim3(EV_THREADS), 0, stream, ctas, args);
-  QE_CHECK_LAUNCH("evict_tokens");
+  const size_t per = ((capacity + ctas - 1) / ctas + 31) / 32 * 32;
+  const int held = per * 4 <= EV_MAX_SMEM;
+  const size_t smem = held ? per * 4 : 0;
+  const dim3 select((unsigned)ctas, (unsigned)(R * Hkv), (unsigned)layers);
+  // a few moves are made by the kernel that lists them: one launch less
   const int most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
-  if (most == 0) return 0;
-  const unsigned blocks = (unsigned)((most + 7) / 8 < 64 ? (most + 7) / 8 : 64);
-  const dim3 grid(blocks, (unsigned)(R * Hkv), (unsigned)layers);
-  if (row_bytes % 16 == 0 && ((uintptr_t)cache & 15) == 0)
-    qe_launch(evict_move_kernel<uint4>, grid, dim3(256), 0, stream, args, (char*)cache, planes, page_size, row_bytes);
-  else if (row_bytes % 4 == 0 && ((uintptr_t)cache & 3) == 0)
-    qe_launch(evict_move_kernel<uint32_t>, grid, dim3(256), 0, stream, args, (char*)cache, planes, page_size, row_bytes);
-  else
-    qe_launch(evict_move_kernel<uint16_t>, grid, dim3(256), 0, stream, args, (char*)cache, planes, page_size, row_bytes);
+  const int unit = row_bytes % 16 == 0 && ((uintptr_t)cache & 15) == 0 ? 16 : (row_bytes % 4 == 0 && ((uintptr_t)cache & 3) == 0 ? 4 : 2);
+  const bool inside = most <= EV_MOVES_INSIDE;
+  cudaError_t e;
+  if (!inside) e = ev_select<0>(select, smem, stream, args, held);
+  else if (unit == 16) e = ev_select<16>(select, smem, stream, args, held);
+  else if (unit == 4) e = ev_select<4>(select, smem, stream, args, held);
+  else e = ev_select<2>(select, smem, stream, args, held);
+  if (e == cudaSuccess && !inside) {
+    const unsigned blocks = (unsigned)((most + 31) / 32 < 64 ? (most + 31) / 32 : 64);
+    const dim3 grid(blocks, (unsigned)(R * Hkv), (unsigned)layers);
+    if (unit == 16) e = qe_launch(evict_move_kernel<uint4>, grid, dim3(256), 0, stream, args);
+    else if (unit == 4) e = qe_launch(evict_move_kernel<uint32_t>, grid, dim3(256), 0, stream, args);
+    else e = qe_launch(evict_move_kernel<uint16_t>, grid, dim3(256), 0, stream, args);
+  }
+  if (e != cudaSuccess) { qe_set_error("evict_tokens: launch failed: %s", cudaGetErrorString(e)); (void)cudaGetLastError(); return 2; }
   QE_CHECK_LAUNCH("evict_tokens");
   return 0;
 }
