@@ -13,15 +13,15 @@
 // entries of every CTA are at the threshold, of which the lowest places stay.  Everybody's place in the lists of movers and of
 // free places then follows from ballots in the order of the entries, a warp a run of them.
 //
-// What bounds it: moving bulk, the copies (an entry's planes are 16 bytes a lane, four entries of a warp on their way at a time); a
+// What bounds it: moving bulk, the copies (16 bytes a lane, four entries of a warp on their way); a
 // step's eviction of an entry, the chain of meetings.
 #include "common.cuh"
 #include <math.h>
 
-#define EV_THREADS 512
-#define EV_WARPS (EV_THREADS / 32)
 #define EV_MAX_CTAS 8
 #define EV_PER_CTA 4096          // entries of a head from which one more CTA joins its cluster
+#define EV_SHORT 6144            // entries of a CTA up to which it has 256 threads ...
+#define EV_MEDIUM 24576          // ... and up to which it has 512
 #define EV_MAX_SMEM (200 * 1024)
 #define EV_MOVES_INSIDE 64       // moves of a head, at most, that the selecting kernel makes itself
 
@@ -46,9 +46,10 @@ __device__ __forceinline__ int ev_ld_remote(const int* local, int cta) {
   return v;
 }
 
-// The keys and values of moves first, first + step, .. below n: a warp an entry, V what one lane moves at a time, four entries on their way.
+// The keys and values of the moves below n, a warp `batch` (32 at most) of them at a time (batches first, first + step, ..): a lane works out where one comes
+// from and goes to, then the warp copies one after the other, V a lane, four on their way.
 template <typename V>
-__device__ __forceinline__ void ev_move(const EvArgs& A, int layer, int r, int h, const int* moves, int n, int first, int step) {
+__device__ __forceinline__ void ev_move(const EvArgs& A, int layer, int r, int h, const int* moves, int n, int first, int step, int batch) {
   const int* table = A.block_tables + (size_t)r * A.max_blocks;
   const size_t plane_bytes = (size_t)A.Hkv * A.page * A.row_bytes;
   char* base = A.cache + (size_t)layer * A.num_pages * A.planes * plane_bytes + (size_t)h * A.page * A.row_bytes;
@@ -57,40 +58,47 @@ __device__ __forceinline__ void ev_move(const EvArgs& A, int layer, int r, int h
     const int b = at / A.page, p = table[b];
     return p >= 0 && p < A.num_pages ? base + (size_t)p * A.planes * plane_bytes + (size_t)(at - b * A.page) * A.row_bytes : nullptr;
   };
-  for (int i = first; i < n; i += 4 * step) {
-    const V* src[4];
-    V* dst[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      src[e] = nullptr; dst[e] = nullptr;
-      if (i + e * step < n) {
-        char* f = place(__ldcg(moves + 1 + i + e * step));
-        char* t = place(__ldcg(moves + 1 + A.keep + i + e * step));
-        if (f && t) { src[e] = reinterpret_cast<const V*>(f); dst[e] = reinterpret_cast<V*>(t); }
-      }
+  for (int i = first * batch; i < n; i += step * batch) {
+    char *f = nullptr, *t = nullptr;
+    if (lane < batch && i + lane < n) {
+      f = place(__ldcg(moves + 1 + i + lane));
+      t = place(__ldcg(moves + 1 + A.keep + i + lane));
+      if (f == nullptr || t == nullptr) f = t = nullptr;
     }
-    for (int v = lane; v < all; v += 32) {
+    const int m = min(batch, n - i);
+    for (int v = lane; v - lane < all; v += 32) {
       const int pl = v / vecs;
-      const size_t o = (pl * plane_bytes) / sizeof(V) + (v - pl * vecs);
-      V x[4];
+      const size_t o = pl * plane_bytes + (size_t)(v - pl * vecs) * sizeof(V);
+      const bool in = v < all;
+      for (int e = 0; e < m; e += 4) {
+        V x[4];
+        char* dst[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) if (src[e]) x[e] = src[e][o];
+        for (int k = 0; k < 4; ++k) {
+          const char* src = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(f), (e + k) & 31));
+          dst[k] = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(t), (e + k) & 31));
+          if (e + k >= m || !in) dst[k] = nullptr;
+          if (dst[k]) x[k] = *reinterpret_cast<const V*>(src + o);
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) if (src[e]) dst[e][o] = x[e];
+        for (int k = 0; k < 4; ++k)
+          if (dst[k]) *reinterpret_cast<V*>(dst[k] + o) = x[k];
+      }
     }
   }
 }
 
 // held: the keys lie in shared memory (else they are formed again wherever they are looked at).  MOVES: 0 where another kernel moves the
 // entries, else the bytes that a lane moves at a time.
-template <int MOVES>
-__global__ void __launch_bounds__(EV_THREADS)
+template <int MOVES, int EV_THREADS>
+__global__ void __launch_bounds__(EV_THREADS, 1024 / EV_THREADS)
 evict_select_kernel(EvArgs A, int held) {
-  extern __shared__ unsigned keys[];
+  constexpr int EV_WARPS = EV_THREADS / 32;
+  extern __shared__ unsigned keys[];              // the CTA's keys, and behind them a bit for every entry that stays
   __shared__ int hist[2][256];
   __shared__ int s_max[EV_WARPS], s_ties[EV_WARPS], s_holes[EV_WARPS], s_movers[EV_WARPS], warp_tot[8];
   __shared__ int x[3];                          // read by the other CTAs of the cluster: latest position, free places, movers
-  __shared__ int digit_s, above_s;
+  __shared__ int digit_s, above_s, equal_s;
   pdl_launch_dependents();
   pdl_wait();
   const int C = (int)cluster_num_ctas(), rank = (int)cluster_cta_rank();
@@ -137,6 +145,7 @@ evict_select_kernel(EvArgs A, int held) {
   }
   const int recent_from = latest - A.recent;
   auto key_of = [&](int p, float w) { return p < A.first || p > recent_from ? 0xffffffffu : ev_key(w); };
+  unsigned* const bits = keys + per;              // (held only)
   auto key_at = [&](int j) { return held ? keys[j - e0] : key_of(P[j], W[j]); };
   // the keep-th largest key; the first pass forms the keys
   unsigned thr = 0u;
@@ -166,11 +175,11 @@ evict_select_kernel(EvArgs A, int held) {
         if ((key & mask) == thr) atomicAdd(&hs[(key >> shift) & 255u], 1);
       }
     }
-    cluster_sync_all();                           // (of one CTA: its threads)
+    if (C > 1) cluster_sync_all(); else __syncthreads();
     int c = 0, mine[EV_MAX_CTAS];
     if (tid < 256) {
 #pragma unroll
-      for (int o = 0; o < EV_MAX_CTAS; ++o) mine[o] = o < C ? ev_ld_remote(&hs[255 - tid], o) : 0;
+      for (int o = 0; o < EV_MAX_CTAS; ++o) mine[o] = C == 1 ? (o == 0 ? hs[255 - tid] : 0) : (o < C ? ev_ld_remote(&hs[255 - tid], o) : 0);
 #pragma unroll
       for (int o = 0; o < EV_MAX_CTAS; ++o) c += mine[o];
       hist[(pass & 1) ^ 1][tid] = 0;              // everybody has read it: they are past this pass's meeting
@@ -188,6 +197,7 @@ evict_select_kernel(EvArgs A, int held) {
       if (run >= left && run - c < left) {
         digit_s = 255 - tid;
         above_s = run - c;
+        equal_s = c;
         int before = 0;                           // (last pass: entries at the threshold in the CTAs before this one)
 #pragma unroll
         for (int o = 0; o < EV_MAX_CTAS; ++o) if (o < rank) before += mine[o];
@@ -202,25 +212,34 @@ evict_select_kernel(EvArgs A, int held) {
   // `left` of the entries at the threshold stay, the lowest places.  A warp has a run of entries: its ties, then its free places and movers, then the lists.
   const int run_len = (per / 32 + EV_WARPS - 1) / EV_WARPS * 32;
   const int j0 = min(e1, e0 + warp * run_len), j1 = min(e1, j0 + run_len);
-  int n = 0;
-  for (int j = j0; j < j1; j += 32) n += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && key_at(j + lane) == thr));
-  if (lane == 0) s_ties[warp] = n;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) ties_before += s_ties[w];
+  const bool choose = equal_s != left;            // (else every entry at the threshold stays, which is the rule but for equal weights)
+  if (choose) {
+    int n = 0;
+    for (int j = j0; j < j1; j += 32) n += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && key_at(j + lane) == thr));
+    if (lane == 0) s_ties[warp] = n;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) ties_before += s_ties[w];
+  }
   const unsigned below = (1u << lane) - 1u;
   // what the 32 entries from j on do: which stay, with `ties` the ties before them
   auto stay = [&](int j, int& ties) {
-    const unsigned key = j + lane < j1 ? key_at(j + lane) : 0u;
-    const unsigned same = __ballot_sync(0xffffffffu, j + lane < j1 && key == thr);
-    const bool s = j + lane < j1 && (key > thr || (key == thr && ties + __popc(same & below) < left));
+    const bool in = j + lane < j1;
+    const unsigned key = in ? key_at(j + lane) : 0u;
+    if (!choose) return in && key >= thr;
+    const unsigned same = __ballot_sync(0xffffffffu, in && key == thr);
+    const bool s = in && (key > thr || (key == thr && ties + __popc(same & below) < left));
     ties += __popc(same);
     return s;
   };
   int holes = 0, movers = 0, ties = ties_before;
   for (int j = j0; j < j1; j += 32) {
-    const bool s = stay(j, ties);
-    holes += __popc(__ballot_sync(0xffffffffu, !s && j + lane < min(j1, keep)));
-    movers += __popc(__ballot_sync(0xffffffffu, s && j + lane >= keep));
+    const unsigned sb = __ballot_sync(0xffffffffu, stay(j, ties));
+    if (held && lane == 0) bits[(j - e0) >> 5] = sb;
+    // of the 32 entries, those before place `keep`
+    const unsigned head = j + 32 <= keep ? 0xffffffffu : (j >= keep ? 0u : (1u << (keep - j)) - 1u);
+    const unsigned valid = j + 32 <= j1 ? 0xffffffffu : (1u << (j1 - j)) - 1u;
+    holes += __popc(~sb & head & valid);
+    movers += __popc(sb & ~head);
   }
   if (lane == 0) { s_holes[warp] = holes; s_movers[warp] = movers; }
   __syncthreads();
@@ -246,15 +265,35 @@ evict_select_kernel(EvArgs A, int held) {
     }
   }
   if (rank == 0 && tid == 0) moves[0] = all_movers;
+  // The kept entries that do not move, where the outputs are other tensors: on their way while the lists are written.
+  if (held && Wo != W) {
+    for (int j = e0 + tid; j < min(e1, keep); j += 4 * EV_THREADS) {
+      float w[4];
+      int p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i * EV_THREADS < min(e1, keep)) { w[i] = W[j + i * EV_THREADS]; p[i] = P[j + i * EV_THREADS]; }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = j + i * EV_THREADS;
+        if (at < min(e1, keep) && ((bits[(at - e0) >> 5] >> ((at - e0) & 31)) & 1u)) {
+          Wo[at] = w[i];
+          if (Po != P) Po[at] = p[i];
+        }
+      }
+    }
+  }
   ties = ties_before;
   for (int j = j0; j < j1; j += 32) {
-    const bool s = stay(j, ties), in = j + lane < j1;
-    const unsigned hb = __ballot_sync(0xffffffffu, !s && j + lane < min(j1, keep)), mb = __ballot_sync(0xffffffffu, s && j + lane >= keep);
+    const unsigned sb = held ? bits[(j - e0) >> 5] : __ballot_sync(0xffffffffu, stay(j, ties));
+    const unsigned head = j + 32 <= keep ? 0xffffffffu : (j >= keep ? 0u : (1u << (keep - j)) - 1u);
+    const unsigned valid = j + 32 <= j1 ? 0xffffffffu : (1u << (j1 - j)) - 1u;
+    const unsigned hb = ~sb & head & valid, mb = sb & ~head;
     if ((hb >> lane) & 1u) moves[1 + keep + holes + __popc(hb & below)] = j + lane;
     if ((mb >> lane) & 1u) moves[1 + movers + __popc(mb & below)] = j + lane;
     holes += __popc(hb);
     movers += __popc(mb);
-    if (in && s && j + lane < keep) {
+    if (!(held && Wo != W) && ((sb & head) >> lane) & 1u) {
       if (Wo != W) Wo[j + lane] = W[j + lane];
       if (Po != P) Po[j + lane] = P[j + lane];
     }
@@ -266,30 +305,37 @@ evict_select_kernel(EvArgs A, int held) {
     Wo[to] = W[from];
     Po[to] = P[from];
   }
-  if (MOVES == 16) ev_move<uint4>(A, layer, r, h, moves, all_movers, rank * EV_WARPS + warp, C * EV_WARPS);
-  if (MOVES == 4) ev_move<uint32_t>(A, layer, r, h, moves, all_movers, rank * EV_WARPS + warp, C * EV_WARPS);
-  if (MOVES == 2) ev_move<uint16_t>(A, layer, r, h, moves, all_movers, rank * EV_WARPS + warp, C * EV_WARPS);
+  if (MOVES == 16) ev_move<uint4>(A, layer, r, h, moves, all_movers, warp * C + rank, C * EV_WARPS, 4);
+  if (MOVES == 4) ev_move<uint32_t>(A, layer, r, h, moves, all_movers, warp * C + rank, C * EV_WARPS, 4);
+  if (MOVES == 2) ev_move<uint16_t>(A, layer, r, h, moves, all_movers, warp * C + rank, C * EV_WARPS, 4);
 }
 
 template <typename V>
 __global__ void __launch_bounds__(256)
-evict_move_kernel(EvArgs A) {
+evict_move_kernel(EvArgs A, int batch) {
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.y / A.Hkv, h = blockIdx.y - r * A.Hkv, layer = blockIdx.z;
   const int* moves = A.moves + (((size_t)layer * A.R + r) * A.Hkv + h) * (size_t)(1 + 2 * A.keep);
-  ev_move<V>(A, layer, r, h, moves, moves[0], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
+  ev_move<V>(A, layer, r, h, moves, moves[0], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8, batch);
 }
 
-template <int MOVES>
-static cudaError_t ev_select(dim3 grid, size_t smem, cudaStream_t stream, const EvArgs& args, int held) {
+template <int MOVES, int THREADS>
+static cudaError_t ev_select_with(dim3 grid, size_t smem, cudaStream_t stream, const EvArgs& args, int held) {
   static bool configured = false;
   if (smem > 48 * 1024 && !configured) {
-    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<MOVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_SMEM);
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<MOVES, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_SMEM);
     if (e != cudaSuccess) return e;
     configured = true;
   }
-  return qe_launch_cluster(evict_select_kernel<MOVES>, grid, dim3(EV_THREADS), smem, stream, grid.x, args, held);
+  return qe_launch_cluster(evict_select_kernel<MOVES, THREADS>, grid, dim3(THREADS), smem, stream, grid.x, args, held);
+}
+// Threads of a CTA: 256 for short runs of entries (four CTAs an SM take turns at their meetings), 512 or 1 024 for long ones.
+template <int MOVES>
+static cudaError_t ev_select(dim3 grid, size_t smem, cudaStream_t stream, const EvArgs& args, int held, long per) {
+  if (per <= EV_SHORT) return ev_select_with<MOVES, 256>(grid, smem, stream, args, held);
+  if (per <= EV_MEDIUM) return ev_select_with<MOVES, 512>(grid, smem, stream, args, held);
+  return ev_select_with<MOVES, 1024>(grid, smem, stream, args, held);
 }
 
 extern "C" int qe_evict_tokens(void* cache, int layers, int num_pages, int planes, int Hkv, int page_size, int row_bytes,
@@ -301,27 +347,32 @@ extern "C" int qe_evict_tokens(void* cache, int layers, int num_pages, int plane
   if ((long)R * Hkv > 65535 || layers > 65535) QE_REFUSE("evict_tokens: %d requests of %d heads, %d layers are more than a launch takes", R, Hkv, layers);
   EvArgs args{block_tables, max_blocks, num_pages, slot_ids, lens, weights, positions, weights_out, positions_out, head_stride,
               slots, Hkv, R, capacity, keep, first, recent, (char*)cache, planes, page_size, row_bytes, moves};
+  // CTAs a head: one, where the heads of all layers and requests are as many as the SMs (a cluster's meetings cost more than a longer run of
+  // entries: 128 heads of 32 768 entries, 8 CTAs each 90 us), else up to EV_MAX_CTAS; and as many as hold the keys
   unsigned ctas = 1;
-  while (ctas < EV_MAX_CTAS && (long)ctas * EV_PER_CTA < capacity) ctas *= 2;
+  const long heads = (long)R * Hkv * layers;
+  while (ctas < EV_MAX_CTAS && ((heads * ctas < 148 && (long)ctas * EV_PER_CTA < capacity) || (long)capacity * 33 / 8 > (long)ctas * (EV_MAX_SMEM - 256))) ctas *= 2;
   const size_t per = ((capacity + ctas - 1) / ctas + 31) / 32 * 32;
-  const int held = per * 4 <= EV_MAX_SMEM;
-  const size_t smem = held ? per * 4 : 0;
+  const int held = per * 4 + per / 8 <= EV_MAX_SMEM;
+  const size_t smem = held ? per * 4 + per / 8 : 0;
   const dim3 select((unsigned)ctas, (unsigned)(R * Hkv), (unsigned)layers);
   // a few moves are made by the kernel that lists them: one launch less
   const int most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
   const int unit = row_bytes % 16 == 0 && ((uintptr_t)cache & 15) == 0 ? 16 : (row_bytes % 4 == 0 && ((uintptr_t)cache & 3) == 0 ? 4 : 2);
   const bool inside = most <= EV_MOVES_INSIDE;
   cudaError_t e;
-  if (!inside) e = ev_select<0>(select, smem, stream, args, held);
-  else if (unit == 16) e = ev_select<16>(select, smem, stream, args, held);
-  else if (unit == 4) e = ev_select<4>(select, smem, stream, args, held);
-  else e = ev_select<2>(select, smem, stream, args, held);
+  if (!inside) e = ev_select<0>(select, smem, stream, args, held, (long)per);
+  else if (unit == 16) e = ev_select<16>(select, smem, stream, args, held, (long)per);
+  else if (unit == 4) e = ev_select<4>(select, smem, stream, args, held, (long)per);
+  else e = ev_select<2>(select, smem, stream, args, held, (long)per);
   if (e == cudaSuccess && !inside) {
-    const unsigned blocks = (unsigned)((most + 31) / 32 < 64 ? (most + 31) / 32 : 64);
+    // moves of a warp at a time: 32, where that still gives every SM 16 warps, else 4
+    const int batch = heads * most >= 148L * 16 * 32 ? 32 : 4;
+    const unsigned blocks = (unsigned)((most + 8 * batch - 1) / (8 * batch) < 64 ? (most + 8 * batch - 1) / (8 * batch) : 64);
     const dim3 grid(blocks, (unsigned)(R * Hkv), (unsigned)layers);
-    if (unit == 16) e = qe_launch(evict_move_kernel<uint4>, grid, dim3(256), 0, stream, args);
-    else if (unit == 4) e = qe_launch(evict_move_kernel<uint32_t>, grid, dim3(256), 0, stream, args);
-    else e = qe_launch(evict_move_kernel<uint16_t>, grid, dim3(256), 0, stream, args);
+    if (unit == 16) e = qe_launch(evict_move_kernel<uint4>, grid, dim3(256), 0, stream, args, batch);
+    else if (unit == 4) e = qe_launch(evict_move_kernel<uint32_t>, grid, dim3(256), 0, stream, args, batch);
+    else e = qe_launch(evict_move_kernel<uint16_t>, grid, dim3(256), 0, stream, args, batch);
   }
   if (e != cudaSuccess) { qe_set_error("evict_tokens: launch failed: %s", cudaGetErrorString(e)); (void)cudaGetLastError(); return 2; }
   QE_CHECK_LAUNCH("evict_tokens");
