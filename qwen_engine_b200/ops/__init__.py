@@ -1674,11 +1674,40 @@ def copy_pages(cache: torch.Tensor, pairs: torch.Tensor) -> None:
                                _stream()), "copy_pages")
 
 
-def _here(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Launches go to the current device's stream: the operands must live there."""
+def _operands(name: str, *tensors: Optional[torch.Tensor]) -> list:
+    """The operands' addresses (None for None), all of them on the current device, whose stream launches go to."""
+    here, out = None, []
     for t in tensors:
-        if t is not None and t.is_cuda and t.device.index != _current_device():
-            raise KernelRefused(f"{name}: a tensor on {t.device} while the current device is cuda:{_current_device()}")
+        if t is None:
+            out.append(None)
+            continue
+        d = t.get_device()
+        if d != here:
+            if d < 0:
+                _ptr(t)                          # (it says what it wants)
+            if here is not None or d != _current_device():
+                raise KernelRefused(f"{name}: a tensor on cuda:{d} while the current device is cuda:{_current_device()}")
+            here = d
+        out.append(t.data_ptr())
+    return out
+
+
+_P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long
+_AW_ARGS = [_P, _L, _I, _P, _I, _I, _P, _I] + [_P] * 8 + [_I, _L] + [_I] * 6 + [_F, _F, _P, _P]
+_SIGNATURES = {       # entry points that are called with plain numbers (ctypes converts them by these types)
+    "qe_attention_weights": _AW_ARGS + [_P] + [_I] * 5 + [_P],
+    "qe_attention_weights_few": _AW_ARGS + [_P] + [_I] * 6 + [_P, _L, _P],
+    "qe_attention_weights_tc": _AW_ARGS + [_P, _I, _I, _P, _P, _I, _I, _I, _P],
+    "qe_evict_tokens": [_P] + [_I] * 6 + [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _L] + [_I] * 4 + [_P, _P],
+    "qe_verify_drafts": [_P] * 11 + [_I] * 3 + [_P],
+}
+
+
+def _entry(name: str):
+    fn = getattr(lib(), name)
+    if fn.argtypes is None:
+        fn.argtypes = _SIGNATURES[name]
+    return fn
 
 
 def _same_or_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1760,26 +1789,29 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
           "accumulate_attention: positions must be int32 [slots, Hkv, capacity]")
     _need(counted is None or (counted.dtype == torch.int32 and counted.shape == (R,) and counted.is_contiguous()),
           "accumulate_attention: counted must be int32 [R]")
-    for t, name in ((slopes, "slopes"), (sinks, "sinks")):
-        _need(t is None or (t.dtype == torch.float32 and t.numel() == Hq and t.is_contiguous()), f"accumulate_attention: {name} must be float32 [Hq]")
+    for t in (slopes, sinks):
+        _need(t is None or (t.dtype == torch.float32 and t.numel() == Hq and t.is_contiguous()), "accumulate_attention: slopes and sinks must be float32 [Hq]")
     _need(scale > 0.0 and softcap >= 0.0, "accumulate_attention: the scale must be positive, the cap not negative")
     page = int(kv_pages.shape[3])
     longest = max((q + c for q, c in zip(ctx.q_lens_host, ctx.ctx_lens_host)), default=0)
-    _need(longest <= weights.shape[2], f"accumulate_attention: a request of {longest} tokens in {weights.shape[2]} places")
-    _need(longest <= int(block_tables.shape[1]) * page, f"accumulate_attention: a request of {longest} tokens in {int(block_tables.shape[1])} blocks of {page}")
-    _here("accumulate_attention", qkv, kv_pages, block_tables, weights, out, positions, counted, slopes, sinks, ctx.cu_q)
-    if R == 0 or T == 0:
+    if longest > weights.shape[2] or longest > block_tables.shape[1] * page:
+        raise KernelRefused(f"accumulate_attention: a request of {longest} tokens in {int(block_tables.shape[1])} blocks of {page} and {int(weights.shape[2])} places")
+    pq, pk, pt, pw, po, pn, pc, psl, psi, pcu, pctx, pslot, pstep = _operands(
+        "accumulate_attention", qkv, kv_pages, block_tables, weights, out, positions, counted, slopes, sinks, ctx.cu_q, ctx.ctx_lens, ctx.slot_ids,
+        ctx.positions)
+    if R == 0:
         return
-    max_total = min(int(weights.shape[2]), int(block_tables.shape[1]) * page)
-    G = Hq // Hkv
-    args = (_ptr(qkv), ctypes.c_long(qkv.stride(0)), T, _ptr(kv_pages), int(kv_pages.shape[0]), planes, _ptr(block_tables),
-            int(block_tables.shape[1]), _ptr(ctx.cu_q), _ptr(ctx.ctx_lens), _ptr(ctx.slot_ids), _ptr(counted), _ptr(ctx.positions),
-            _ptr(positions), _ptr(weights), _ptr(out), int(weights.shape[0]), ctypes.c_long(weights.shape[2]), R, Hq, Hkv, D, page,
-            int(window), ctypes.c_float(scale), ctypes.c_float(softcap), _ptr(slopes), _ptr(sinks))
+    blocks, capacity = block_tables.shape[1], weights.shape[2]
+    max_total, G, max_q = min(capacity, blocks * page), Hq // Hkv, max(ctx.q_lens_host)
+    stream = _stream()
+    args = (pq, qkv.stride(0), T, pk, kv_pages.shape[0], planes, pt, blocks, pcu, pctx, pslot, pc, pstep, pn, pw, po, weights.shape[0], capacity, R,
+            Hq, Hkv, D, page, int(window), scale, softcap, psl, psi)
     # the requests of a few rows, and the others
     few = -1
-    if qkv.dtype == torch.bfloat16 and D % 8 == 0 and D <= 1024 and kv_pages.data_ptr() % 16 == 0:
-        few = max((n * G for n in ctx.q_lens_host if n * G <= ATTENTION_WEIGHTS_FEW_ROWS), default=-1)
+    if qkv.dtype == torch.bfloat16 and D % 8 == 0 and D <= 1024 and pk % 16 == 0:
+        few = max((max(n, 1) * G for n in ctx.q_lens_host if n * G <= ATTENTION_WEIGHTS_FEW_ROWS), default=-1)
+        if few > ATTENTION_WEIGHTS_FEW_ROWS:     # (requests without a token, of more heads than that)
+            few = ATTENTION_WEIGHTS_FEW_ROWS
     if few > 0:
         span = min(max_total, int(window) + few // G + 31) if window > 0 else max_total
         ctas, part_keys = attention_weights_cluster(few, Hkv, D, R, span)
@@ -1787,26 +1819,27 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
         if ctas == 0:
             parts = min(-(-span // part_keys), ATTENTION_WEIGHTS_MAX_PARTS)
             ld = -(-(span + 32) // 32) * 32
-            scores, stats = alloc((R, Hkv, few, ld), torch.float32), alloc((T * Hq, parts, 2), torch.float32)
-        _check(lib().qe_attention_weights_few(*args, _ptr(stats), parts, few, max_total, span, ctas, part_keys, _ptr(scores), ctypes.c_long(ld), _stream()),
-               "accumulate_attention")
-    max_q = max(ctx.q_lens_host)
-    if few >= max_q * G:
-        return
-    if (ATTENTION_WEIGHTS_TC and qkv.dtype == torch.bfloat16 and qkv.data_ptr() % 16 == 0 and qkv.stride(0) % 8 == 0
-            and kv_pages.data_ptr() % 16 == 0 and lib().qe_attention_weights_tc_supported(Hq, Hkv, D, page)):
+            scores, stats = alloc((R, Hkv, few, ld), torch.float32), alloc((max(T, 1) * Hq, parts, 2), torch.float32)
+        _check(_entry("qe_attention_weights_few")(
+            *args, None if stats is None else stats.data_ptr(), parts, few, max_total, span, ctas, part_keys,
+            None if scores is None else scores.data_ptr(), ld, stream), "accumulate_attention")
+        if few >= max_q * G:
+            return
+    if (ATTENTION_WEIGHTS_TC and qkv.dtype == torch.bfloat16 and pq % 16 == 0 and qkv.stride(0) % 8 == 0 and pk % 16 == 0 and max_q > 0
+            and lib().qe_attention_weights_tc_supported(Hq, Hkv, D, page)):
         tpt, na = 128 // G, 4 if D <= 128 else (2 if D <= 192 else 1)      # tokens of a tile of queries, tiles a unit
         many = [(n, n + c) for n, c in zip(ctx.q_lens_host, ctx.ctx_lens_host) if n * G > few]
         parts1 = attention_weights_tc_parts(sum(-(-n // (tpt * na)) for n, _ in many) * Hkv, -(-max_total // 128))
         parts2 = attention_weights_tc_parts(sum(-(-t // (128 * na)) for _, t in many) * Hkv, -(-max_q // tpt))
         stats, merged = alloc((T * Hq, parts1, 2), torch.float32), alloc((Hkv, T // tpt + R, 128), torch.float32)
         sums = alloc((parts2, R, Hkv, max_total), torch.float32) if parts2 > 1 else None
-        _check(lib().qe_attention_weights_tc(*args, _ptr(stats), parts1, parts2, _ptr(merged), _ptr(sums), max_q, max_total, few, _stream()),
-               "accumulate_attention")
+        _check(_entry("qe_attention_weights_tc")(
+            *args, stats.data_ptr(), parts1, parts2, merged.data_ptr(), None if sums is None else sums.data_ptr(), max_q, max_total, few, stream),
+            "accumulate_attention")
     else:
         parts = _attention_weights_parts(-(-max_q * G // 64), Hkv, R, max_total)
-        stats = alloc((T * Hq, parts, 2), torch.float32)
-        _check(lib().qe_attention_weights(*args, _ptr(stats), parts, max_q, max_total, few, _dt(qkv), _stream()), "accumulate_attention")
+        stats = alloc((max(T, 1) * Hq, parts, 2), torch.float32)
+        _check(_entry("qe_attention_weights")(*args, stats.data_ptr(), parts, max_q, max_total, few, _dt(qkv), stream), "accumulate_attention")
 
 
 def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,
@@ -1836,21 +1869,21 @@ def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torc
           "evict_tokens: weights must be contiguous float32 [layers, slots, Hkv, capacity]")
     _need(positions.dtype == torch.int32 and positions.shape == weights.shape and positions.is_contiguous(),
           "evict_tokens: positions must be contiguous int32 [layers, slots, Hkv, capacity]")
-    for t, like, name in ((weights_out, weights, "weights_out"), (positions_out, positions, "positions_out")):
-        _need(t.dtype == like.dtype and t.shape == like.shape and t.is_contiguous(), f"evict_tokens: {name} must be like its input")
-        _need(_same_or_apart(t, like), f"evict_tokens: {name} must be its input or share no memory with it")
+    for t, like in ((weights_out, weights), (positions_out, positions)):
+        _need(t.dtype == like.dtype and t.shape == like.shape and t.is_contiguous(), "evict_tokens: weights_out and positions_out must be like their inputs")
+        _need(_same_or_apart(t, like), "evict_tokens: weights_out and positions_out must be their inputs or share no memory with them")
     _need(int(keep) >= 1 and int(first) >= 0 and int(recent) >= 0, "evict_tokens: keep must be at least 1, first and recent not negative")
-    _need(int(first) + int(recent) <= int(keep), f"evict_tokens: {first} first and {recent} recent entries do not fit a budget of {keep}")
-    _here("evict_tokens", cache, block_tables, slot_ids, lens, weights, positions, weights_out, positions_out)
+    if int(first) + int(recent) > int(keep):
+        raise KernelRefused(f"evict_tokens: {first} first and {recent} recent entries do not fit a budget of {keep}")
+    pc, pt, psl, pl, pw, pp, pwo, ppo = _operands("evict_tokens", cache, block_tables, slot_ids, lens, weights, positions, weights_out, positions_out)
     if R == 0 or S == 0:
         return
-    capacity = min(int(weights.shape[3]), int(block_tables.shape[1]) * page)
+    capacity = min(weights.shape[3], block_tables.shape[1] * page)
     keep = min(int(keep), max(capacity, 1))
     moves = alloc((S, R, Hkv, 1 + 2 * keep), torch.int32)
-    _check(lib().qe_evict_tokens(
-        _ptr(cache), S, pages, planes, Hkv, page, D * cache.element_size(), _ptr(block_tables), int(block_tables.shape[1]), _ptr(slot_ids),
-        _ptr(lens), R, _ptr(weights), _ptr(positions), _ptr(weights_out), _ptr(positions_out), int(weights.shape[1]),
-        ctypes.c_long(weights.shape[3]), capacity, keep, int(first), int(recent), _ptr(moves), _stream()), "evict_tokens")
+    _check(_entry("qe_evict_tokens")(
+        pc, S, pages, planes, Hkv, page, D * cache.element_size(), pt, block_tables.shape[1], psl, pl, R, pw, pp, pwo, ppo, weights.shape[1],
+        weights.shape[3], capacity, keep, int(first), int(recent), moves.data_ptr(), _stream()), "evict_tokens")
 
 
 def silu_mul(gate_up: torch.Tensor, out: torch.Tensor) -> None:
@@ -2595,20 +2628,17 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, draft_logits
     N, V = logits.shape
     R = counts.numel()
     _need(logits.dtype == torch.float32 and logits.is_contiguous(), "verify_drafts: logits must be contiguous float32 [N, V]")
-    for t, n, name in ((draft_tokens, N - R, "draft_tokens"), (row_starts, R + 1, "row_starts"), (top_k, R, "top_k"), (tokens, N, "tokens"),
-                       (counts, R, "counts")):
-        _i32(t, f"verify_drafts: {name}")
-        _need(t.numel() == n, f"verify_drafts: {name} has {t.numel()} entries, not {n}")
-    for t, n, name in ((temperature, R, "temperature"), (uniform, N, "uniform")):
-        _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, f"verify_drafts: {name} must be float32 with {n} entries")
+    for t, n in ((draft_tokens, N - R), (row_starts, R + 1), (top_k, R), (tokens, N), (counts, R)):
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
+              "verify_drafts: draft_tokens [N - R], row_starts [R + 1], top_k [R], tokens [N] and counts [R] must be contiguous int32")
+    for t, n in ((temperature, R), (uniform, N)):
+        _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, "verify_drafts: temperature [R] and uniform [N] must be contiguous float32")
     _need(draft_logits is None or (draft_logits.dtype == torch.float32 and draft_logits.is_contiguous() and draft_logits.shape == (N - R, V)),
           "verify_drafts: draft_logits must be contiguous float32 [N - R, V]")
-    _here("verify_drafts", logits, draft_tokens, draft_logits, row_starts, temperature, top_k, uniform, tokens, counts)
+    addresses = _operands("verify_drafts", logits, draft_tokens, draft_logits if N > R else None, row_starts, temperature, top_k, uniform, tokens, counts)
     if R == 0:
         return
     rows = N + (N - R if draft_logits is not None else 0)
     parts = alloc((rows, VERIFY_CHUNKS, 2), torch.float64)        # 16 bytes a chunk: sum, maximum, its place
     thresholds = alloc((rows,), torch.int32)
-    _check(lib().qe_verify_drafts(_ptr(logits), _ptr(draft_tokens), _ptr(draft_logits if N > R else None), _ptr(row_starts), _ptr(temperature),
-                                  _ptr(top_k), _ptr(uniform), _ptr(tokens), _ptr(counts), _ptr(parts), _ptr(thresholds), N, R, V, _stream()),
-           "verify_drafts")
+    _check(_entry("qe_verify_drafts")(*addresses, parts.data_ptr(), thresholds.data_ptr(), N, R, V, _stream()), "verify_drafts")

@@ -582,3 +582,12 @@ def test_accumulate_attention_on_the_tensor_cores_with_every_option():
             _check_weights(c, window=100, sinks=torch.randn(Hq), softcap=4.0, slopes=torch.rand(Hq) * 0.1)
             _check_weights(c, window=1, sinks=torch.randn(Hq))
             _check_weights(c, window=129, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_accumulate_attention_of_requests_without_tokens(dtype):
+    """A request that brings nothing keeps what its keys have gathered, beside others and alone."""
+    for q_lens, ctx_lens in (([0, 2], [70, 9]), ([0, 90], [300, 5]), ([0], [40])):
+        c = _weights_case(dtype, 4, 2, 64, 16, q_lens, ctx_lens, 95)
+        c["qkv"] = c["qkv"] if sum(q_lens) else torch.zeros(0, 8 * 64, dtype=dtype)
+        _check_weights(c)

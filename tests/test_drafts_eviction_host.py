@@ -122,3 +122,16 @@ def test_where_a_few_rows_scores_go():
         for tiles in (1, 3, 4, 100):
             parts = ops.attention_weights_tc_parts(units, tiles)
             assert 1 <= parts <= max(1, -(-tiles // 4)) and (parts == 1 or (parts - 1) * units < 4 * 148)
+
+
+def test_the_entry_points_take_what_the_fronts_give():
+    """The types by which ctypes converts the arguments, against the entry points' declarations."""
+    import os
+    import re
+    folder = os.path.join(os.path.dirname(os.path.abspath(ops.__file__)), "..", "csrc")
+    source = "".join(open(os.path.join(folder, f)).read() for f in sorted(os.listdir(folder)) if f.endswith(".cu"))
+    for name, types in ops._SIGNATURES.items():
+        declared = re.search(r'extern "C" int ' + name + r"\(([^)]*)\)", source).group(1).split(",")
+        kinds = [ops._P if "*" in d or "cudaStream_t" in d else ops._L if d.strip().startswith("long ") else ops._F if d.strip().startswith("float ") else ops._I
+                 for d in declared]
+        assert kinds == types, name
