@@ -70,3 +70,6 @@ __device__ __forceinline__ float2 aw_merge(const float* st, int parts, const flo
   if (sink) z += exp2f(*sink * AW_LOG2E - m);
   return make_float2(m, 1.f / z);
 }
+
+// Adds the parts of the keys' sums ([parts, R, Hkv, ld]) up, in their order, and writes the output of the requests of more than few_rows rows (attention_weights.cu).
+cudaError_t aw_finish(const AwArgs& A, const float* sums, long ld, int parts, int few_rows, int max_total, cudaStream_t stream);

@@ -437,21 +437,6 @@ attention_weights_merge_kernel(AwArgs A, AwTc C) {
   C.negl[((size_t)c * C.tiles + at2_tile0(R, r, C.tpt) + tile) * AT2_TILE + rr] = v;
 }
 
-__global__ void __launch_bounds__(256)
-attention_weights_finish_kernel(AwArgs A, AwTc C) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int c = blockIdx.y, r = blockIdx.z, k = blockIdx.x * 256 + threadIdx.x;
-  const AwReq R = aw_req(A, r);
-  const int slot = A.slot_ids[r];
-  if ((long)R.n * (A.Hq / A.Hkv) <= C.few_rows || k >= R.total || slot < 0 || slot >= A.slots) return;
-  float total = 0.f;
-  for (int p = 0; p < C.parts; ++p) total += C.sums[(((size_t)p * A.R + r) * A.Hkv + c) * C.sums_ld + k];
-  const size_t at = ((size_t)slot * A.Hkv + c) * A.capacity + k;
-  A.out[at] = k < R.ctx ? A.weights[at] + total : total;
-  if (A.positions && k >= R.ctx) A.positions[at] = A.step_positions[R.row0 + k - R.ctx];
-}
-
 extern "C" int qe_attention_weights_tc_status() {
   int v = 0;
   cudaMemcpyFromSymbol(&v, g_awtc_status, sizeof(int));
@@ -535,7 +520,7 @@ extern "C" int qe_attention_weights_tc(const void* q, long q_stride, int T, cons
   C.parts = parts2;
   if (e == cudaSuccess) e = general ? at2_launch<2, true>(grid2, stream, map_q, map_k, A, C) : at2_launch<2, false>(grid2, stream, map_q, map_k, A, C);
   if (e == cudaSuccess && C.sums)
-    e = qe_launch(attention_weights_finish_kernel, dim3((unsigned)((max_total + 255) / 256), (unsigned)Hkv, (unsigned)R), dim3(256), 0, stream, A, C);
+    e = aw_finish(A, C.sums, C.sums_ld, parts2, few_rows, max_total, stream);
   if (e != cudaSuccess) { qe_set_error("attention_weights: launch failed: %s", cudaGetErrorString(e)); (void)cudaGetLastError(); return 2; }
   QE_CHECK_LAUNCH("attention_weights");
   return 0;

@@ -1695,7 +1695,7 @@ def _operands(name: str, *tensors: Optional[torch.Tensor]) -> list:
 _P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long
 _AW_ARGS = [_P, _L, _I, _P, _I, _I, _P, _I] + [_P] * 8 + [_I, _L] + [_I] * 6 + [_F, _F, _P, _P]
 _SIGNATURES = {       # entry points that are called with plain numbers (ctypes converts them by these types)
-    "qe_attention_weights": _AW_ARGS + [_P] + [_I] * 5 + [_P],
+    "qe_attention_weights": _AW_ARGS + [_P] + [_I] * 5 + [_P, _I, _P],
     "qe_attention_weights_few": _AW_ARGS + [_P] + [_I] * 6 + [_P, _L, _P],
     "qe_attention_weights_tc": _AW_ARGS + [_P, _I, _I, _P, _P, _I, _I, _I, _P],
     "qe_evict_tokens": [_P] + [_I] * 6 + [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _L] + [_I] * 4 + [_P, _P],
@@ -1719,9 +1719,9 @@ def _same_or_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
 ATTENTION_WEIGHTS_MAX_PARTS = 64      # parts of a row's keys at most, where the rows alone do not fill the SMs
 
 
-def _attention_weights_parts(row_tiles: int, heads: int, requests: int, max_total: int) -> int:
-    """In how many parts the rows' keys are cut: two CTAs an SM, and 256 keys a part at least."""
-    return max(1, min(-(-FLASH_TARGET_CTAS // max(1, row_tiles * heads * requests)), -(-max_total // 256), ATTENTION_WEIGHTS_MAX_PARTS))
+def _attention_weights_parts(ctas: int, tiles: int) -> int:
+    """In how many parts the other side's tiles are cut where one CTA each would be ``ctas``: four CTAs an SM, a tile a part at least."""
+    return max(1, min(-(-4 * TC_TARGET_CTAS // max(1, ctas)), tiles, ATTENTION_WEIGHTS_MAX_PARTS))
 
 
 ATTENTION_WEIGHTS_FEW_ROWS = 32               # rows of a request (a query token x a query head of a kv head's group) up to which the kernel of few rows serves
@@ -1837,9 +1837,12 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
             *args, stats.data_ptr(), parts1, parts2, merged.data_ptr(), None if sums is None else sums.data_ptr(), max_q, max_total, few, stream),
             "accumulate_attention")
     else:
-        parts = _attention_weights_parts(-(-max_q * G // 64), Hkv, R, max_total)
+        rows, keys = -(-max_q * G // 64), -(-max_total // 64)          # tiles of either, about
+        parts, parts2 = _attention_weights_parts(rows * Hkv * R, keys), _attention_weights_parts(keys * Hkv * R, rows)
         stats = alloc((max(T, 1) * Hq, parts, 2), torch.float32)
-        _check(_entry("qe_attention_weights")(*args, stats.data_ptr(), parts, max_q, max_total, few, _dt(qkv), stream), "accumulate_attention")
+        sums = alloc((parts2, R, Hkv, max_total), torch.float32) if parts2 > 1 else None
+        _check(_entry("qe_attention_weights")(
+            *args, stats.data_ptr(), parts, max_q, max_total, few, parts2, None if sums is None else sums.data_ptr(), _dt(qkv), stream), "accumulate_attention")
 
 
 def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,

@@ -101,10 +101,10 @@ def test_the_sampler_refuses_lists_that_do_not_fit():
 
 
 def test_parts_of_rows():
-    """Rows that fill the SMs are not cut; a few rows are cut into as many parts of 256 keys as give every SM two CTAs."""
-    assert ops._attention_weights_parts(64, 8, 1, 4096) == 1
-    assert ops._attention_weights_parts(1, 8, 1, 4096) == 16 and ops._attention_weights_parts(1, 8, 1, 131072) == 37
-    assert ops._attention_weights_parts(1, 1, 1, 1 << 20) == ops.ATTENTION_WEIGHTS_MAX_PARTS and ops._attention_weights_parts(1, 1, 1, 1) == 1
+    """Tiles that give every SM four CTAs are not cut; fewer are cut into as many parts as do, of a tile of the other side at least."""
+    assert ops._attention_weights_parts(600, 32) == 1 and ops._attention_weights_parts(592, 32) == 1
+    assert ops._attention_weights_parts(100, 32) == 6 and ops._attention_weights_parts(8, 5) == 5 and ops._attention_weights_parts(1, 0) == 1
+    assert ops._attention_weights_parts(1, 1 << 13) == ops.ATTENTION_WEIGHTS_MAX_PARTS
 
 
 def test_where_a_few_rows_scores_go():
