@@ -146,7 +146,7 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
   __shared__ int owner;
   pdl_launch_dependents();
   pdl_wait();
-  const int C = (int)cluster_num_ctas(), rank = (int)cluster_cta_rank(), y = blockIdx.y;
+  const int C = (int)cluster_num_ctas(), rank = (int)cluster_cta_rank(), y = blockIdx.x / C;
   const bool draft = y >= N;
   const int r = vf_owner(starts, R, draft ? y - N : y, draft ? 1 : 0, &owner);
   const float T = temperature[r];
@@ -412,7 +412,7 @@ verify_draw_kernel(const float* __restrict__ logits, const float* __restrict__ d
   if (threadIdx.x < 32) pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
   pdl_launch_dependents();
   pdl_wait();
-  const int C = (int)cluster_num_ctas(), rank = (int)cluster_cta_rank(), r = blockIdx.y;
+  const int C = (int)cluster_num_ctas(), rank = (int)cluster_cta_rank(), r = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int D = N - R;
   const int lo = min(max(starts[r], 0), N), hi = min(max(starts[r + 1], lo), N);
@@ -636,7 +636,7 @@ extern "C" int qe_verify_drafts(const float* logits, const int* draft_tokens, co
   if (V <= 0) QE_REFUSE("verify_drafts: empty vocabulary");
   if (N < R) QE_REFUSE("verify_drafts: %d rows for %d requests", N, R);
   const long rows = (long)N + (draft_logits ? N - R : 0);
-  if (rows > 65535 || R > 65535) QE_REFUSE("verify_drafts: %ld rows are more than a launch takes (65535)", rows);
+  if (rows > 0x7fffffffL / VF_MAX_DRAW) QE_REFUSE("verify_drafts: %ld rows are more than a launch takes", rows);
   // CTAs a row: three rounds of the CTAs that the SMs hold at once, so that a CTA reads a long run of a row where there are many rows;
   // a request to draw for: a CTA an SM.  (Always eight: 64 requests of five drafts, 151 936 logits, 228 us for the first kernel.)
   unsigned ctas = 1, draw = 1;
@@ -650,10 +650,10 @@ extern "C" int qe_verify_drafts(const float* logits, const int* draft_tokens, co
       configured = true;
     }
   }
-  qe_launch_cluster(verify_sums_kernel, dim3(ctas, (unsigned)rows), dim3(VF_THREADS), 0, stream, ctas, logits, draft_logits,
+  qe_launch_cluster(verify_sums_kernel, dim3((unsigned)(rows * ctas)), dim3(VF_THREADS), 0, stream, ctas, logits, draft_logits,
                     starts, temperature, top_k, (VfPart*)parts, thresholds, N, R, V);
   QE_CHECK_LAUNCH("verify_drafts");
-  qe_launch_cluster(verify_draw_kernel, dim3(draw, (unsigned)R), dim3(VF_THREADS), 0, stream, draw, logits, draft_logits,
+  qe_launch_cluster(verify_draw_kernel, dim3((unsigned)R * draw), dim3(VF_THREADS), 0, stream, draw, logits, draft_logits,
                     draft_tokens, starts, temperature, uniform, (const VfPart*)parts, thresholds, tokens, counts, (int)ctas, N, R, V);
   QE_CHECK_LAUNCH("verify_drafts");
   return 0;

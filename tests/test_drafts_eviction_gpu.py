@@ -147,6 +147,27 @@ def test_verified_tokens_are_distributed_as_the_targets(model):
     assert int(tokens[::2].min()) >= 0 and 0.1 < float((counts == 2).double().mean()) < 0.99
 
 
+def test_verify_drafts_of_very_many_requests():
+    """More rows than a grid's second dimension holds: every request is the same one, and so is what it gains."""
+    R, V = 40000, 6
+    c = _verify_case(1, [1], V, 14, True)
+    want = plain_drafts.verify(**c)
+    many = dict(logits=c["logits"].repeat(R, 1), draft_tokens=c["draft_tokens"].repeat(R), draft_logits=c["draft_logits"].repeat(R, 1),
+                row_starts=torch.arange(0, 2 * R + 1, 2, dtype=torch.int32), temperature=c["temperature"].repeat(R), top_k=c["top_k"].repeat(R),
+                uniform=c["uniform"].repeat(R))
+    tokens, counts = _verify(many)
+    assert (counts == want[1]).all() and (tokens.view(R, 2) == want[0]).all()
+
+
+def test_verify_drafts_with_extreme_temperatures():
+    """Temperatures at which nothing but the largest logits, or all of them alike, have weight; large logits and close ones."""
+    c = _verify_case(12, [2], 257, 15, True)
+    c["temperature"] = torch.tensor([1e-30, 1e-6, 1e-3, 1e3, 1e6, 1e20, 3e38, 1.0, 0.5, -1.0, 1e-38, 2.0])
+    for scale, shift in ((1.0, 0.0), (1e-3, 1e4), (1e6, 0.0), (1e30, 0.0)):
+        d = dict(c, logits=c["logits"] * scale + shift, draft_logits=c["draft_logits"] * scale + shift)
+        _same(_verify(d), plain_drafts.verify(**d))
+
+
 def test_verify_drafts_of_a_request_without_rows():
     """It gets no tokens, and the requests in front of it theirs."""
     c = _verify_case(2, [2], 50, 9, True)
@@ -398,6 +419,11 @@ def test_evict_tokens_with_infinities_and_nan():
 def test_evict_tokens_from_long_caches(lens, keep, first, recent):
     for in_place in (False, True):
         _check_evict(_evict_case(torch.bfloat16, 1, 1, 16, 16, lens, 6, ordered=keep == 1000), keep, first, recent, in_place)
+
+
+def test_evict_tokens_from_a_cache_whose_keys_do_not_fit_on_the_chip():
+    for keep in (300, 409999):
+        _check_evict(_evict_case(torch.bfloat16, 1, 1, 8, 64, [410000], 7, planes=1), keep, 3, 50)
 
 
 def test_evicting_twice_is_evicting_from_what_is_left():
