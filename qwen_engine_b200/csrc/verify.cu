@@ -13,8 +13,8 @@
 // together, holds the drafts against them, and draws.
 //
 // The top_k-th largest logit.  Of a chunk's logits only the k largest can be among the row's k largest, and the k-th largest of
-// the threads' maxima is a lower bound of the chunk's k-th largest: with 512 threads and a k of some tens hardly more than k
-// logits reach it.  The CTAs list theirs, and the k-th largest of the lists (a few hundred numbers, found bit by bit) is the
+// the threads' maxima (of the maxima of either half of their logits, for a k of some hundreds) is a lower bound of the chunk's k-th largest: hardly
+// more than k logits reach it.  The CTAs list theirs, and the k-th largest of the lists (a few hundred numbers, found bit by bit) is the
 // row's.  Where k is large, or the lists overflow (equal logits), the digits of an order-preserving integer are found one
 // after the other from histograms that meet in distributed shared memory.
 //
@@ -98,7 +98,8 @@ __device__ __forceinline__ unsigned vf_ld_remote(const unsigned* local, int cta)
 
 #define VF_LIST 1024         // logits of a chunk that may reach the lower bound
 #define VF_ALL 2048          // ... of a row's chunks together
-#define VF_LIST_K 384        // top_k a chunk up to which the lists are tried (a bound from 512 maxima says little beyond)
+#define VF_RANKED 512        // ... up to which each is compared with every other
+#define VF_LIST_K 768        // top_k a chunk up to which the lists are tried (a bound from 2 x 512 maxima says little beyond)
 #define VF_AHEAD 4           // groups of four logits that a thread asks for at a time
 
 __device__ __forceinline__ float2 vf_add2(float2 a, float2 b) {
@@ -142,6 +143,7 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
   __shared__ __align__(16) unsigned all[VF_ALL + 4];
   __shared__ unsigned digit_s, above_s, listed, bound, found, sizes[VF_MAX_CTAS];
   __shared__ unsigned warp_tot[VF_WARPS];
+  __shared__ int warp_two[2][VF_WARPS];
   __shared__ double sz[VF_WARPS];
   __shared__ int owner;
   pdl_launch_dependents();
@@ -160,7 +162,7 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
   const bool some = !greedy && k > 0 && k < V;  // the row keeps its k largest
   const float c = vf_scale(T);
   // the thread's groups: g0 + tid + i VF_THREADS, the first and the last of the row (which may reach beyond it) with care
-  float m = -FLT_MAX, s = 0.f;
+  float m = -FLT_MAX, s = 0.f, half[2] = {-INFINITY, -INFINITY};      // half: the maxima of every second group, for the bound of a large top_k
   int at = 0x7fffffff;
   if (greedy) m = -INFINITY;
   for (int g = g0 + tid; g < g1; g += VF_AHEAD * VF_THREADS) {
@@ -184,6 +186,7 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
           at = x[i].x == top ? e : (x[i].y == top ? e + 1 : (x[i].z == top ? e + 2 : e + 3));
         }
         m = fmaxf(m, top);
+        half[i & 1] = fmaxf(half[i & 1], top);
       }
     }
   }
@@ -221,9 +224,11 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
       // The high half of the k / C-th largest of the threads' maxima, in every chunk: at least k logits reach the least of those
       // numbers, so it is a lower bound of the row's k-th largest.
       unsigned low = 0u;
+      const unsigned h0 = vf_key(half[0]), h1 = g0 + tid + VF_THREADS < g1 ? vf_key(half[1]) : 0u;
       for (int bit = 31; bit >= 16; --bit) {
         const unsigned cand = low | (1u << bit);
-        if (__syncthreads_count(mine >= cand) >= kc) low = cand;
+        int n = kc <= VF_THREADS / 4 ? __syncthreads_count(mine >= cand) : __syncthreads_count(mine != 0u && h0 >= cand) + __syncthreads_count(h1 >= cand);
+        if (n >= kc) low = cand;
       }
       if (tid == 0) bound = low;
       cluster_sync_all();
@@ -265,19 +270,39 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
       if (from_list && tid < 4) all[total + tid] = 0u;         // (read four at a time below)
       cluster_sync_all();                       // the lists have been read
       if (from_list) {
-        // the k-th largest: the one with fewer than k above it and at least k with its equals
-        for (unsigned i = tid; i < total; i += VF_THREADS) {
-          const unsigned key = all[i];
-          int above = 0, equal = 0;
-          for (unsigned j = 0; j < total; j += 4) {
-            const uint4 o = *reinterpret_cast<const uint4*>(all + j);
-            above += (o.x > key) + (o.y > key) + (o.z > key) + (o.w > key);
-            equal += (o.x == key) + (o.y == key) + (o.z == key) + (o.w == key);
+        if (total <= VF_RANKED) {
+          // the k-th largest: the one with fewer than k above it and at least k with its equals
+          if (tid < total) {
+            const unsigned key = all[tid];
+            int above = 0, equal = 0;
+            for (unsigned j = 0; j < total; j += 4) {
+              const uint4 o = *reinterpret_cast<const uint4*>(all + j);
+              above += (o.x > key) + (o.y > key) + (o.z > key) + (o.w > key);
+              equal += (o.x == key) + (o.y == key) + (o.z == key) + (o.w == key);
+            }
+            if (above < k && above + equal >= k) found = key;
           }
-          if (above < k && above + equal >= k) found = key;
+          __syncthreads();
+          thr = found;
+        } else {
+          // bit by bit
+          unsigned keys[VF_ALL / VF_THREADS];
+#pragma unroll
+          for (int i = 0; i < VF_ALL / VF_THREADS; ++i) keys[i] = (unsigned)(i * VF_THREADS + tid) < total ? all[i * VF_THREADS + tid] : 0u;
+          for (int bit = 31; bit >= 0; --bit) {
+            const unsigned cand = thr | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < VF_ALL / VF_THREADS; ++i) n += keys[i] >= cand;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (lane == 0) warp_two[bit & 1][warp] = n;         // (two in turn: one meeting a bit)
+            __syncthreads();
+            n = 0;
+#pragma unroll
+            for (int w = 0; w < VF_WARPS; ++w) n += warp_two[bit & 1][w];
+            if (n >= k) thr = cand;
+          }
         }
-        __syncthreads();
-        thr = found;
         for (unsigned i = tid; i < listed; i += VF_THREADS)      // (the chunk's kept logits are in its list)
           if (list[i] >= thr) {
             const float x = vf_unkey(list[i]);
