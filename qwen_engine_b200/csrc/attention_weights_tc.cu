@@ -13,9 +13,11 @@
 // pass, in their order, so sums do not depend on which CTA was first.  Between the passes it leaves -log2 of every row's whole
 // sum, exponentials and maximum together, in the order of the second pass's columns: a weight is then one exponential.
 //
-// What bounds it: a product of 128 x 128 x 128 takes the tensor cores 512 cycles and its 16 384 exponentials the
-// special-function unit 1 024.  So a quarter of the exponentials is a polynomial (at2_poly2), two at a time on the float32 units: more
-// of them cost the readers more instructions than the special-function unit gains.
+// What bounds it: a product of 128 x 128 x 128 takes the tensor cores 512 cycles at best (both operands from shared memory, 8 KB every 64 cycles, are
+// all that it delivers; measured, with the readers beside it, about 950), its 16 384 exponentials the special-function unit 1 024, and the
+// readers' instructions their issue slots about as long.  An eighth of the exponentials is a polynomial (at2_poly2), two at a time on the float32
+// units: none 256, an eighth 249, a quarter 259, three eighths 271 us for a prompt of 4 096 tokens with 32 / 8 heads (one CTA walking several
+// units 269: some are empty, and they are dealt out beforehand).
 //
 // Every wait is bounded: one that runs out records a code, raises the CTA's abort flag, and the CTA leaves without writing.
 #include "attention_weights.cuh"
@@ -93,7 +95,7 @@ __device__ __forceinline__ float2 at2_poly2(float2 x) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 // whether the pair of columns 2 j, 2 j + 1 of a chunk goes there
-__device__ constexpr bool at2_on_poly(int j) { return (j & 3) == 1; }
+__device__ constexpr bool at2_on_poly(int j) { return (j & 7) == 1; }
 __device__ __forceinline__ float2 at2_exp2(float2 x, bool poly) { return poly ? at2_poly2(x) : make_float2(at2_ex2(x.x), at2_ex2(x.y)); }
 
 // one thread's share of the first pass: its row's running maximum and sum, and the keys it may see
