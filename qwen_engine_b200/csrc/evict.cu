@@ -93,7 +93,7 @@ __device__ __forceinline__ void ev_move(const EvArgs& A, int layer, int r, int h
 template <int MOVES, int EV_THREADS>
 __global__ void __launch_bounds__(EV_THREADS, 1024 / EV_THREADS)
 evict_select_kernel(EvArgs A, int held) {
-  constexpr int EV_WARPS = EV_THREADS / 32;
+  constexpr int EV_WARPS = EV_THREADS / 32, AHEAD = EV_THREADS <= 512 ? 8 : 4;      // AHEAD: loads of a thread on their way
   extern __shared__ unsigned keys[];              // the CTA's keys, and behind them a bit for every entry that stays
   __shared__ int hist[2][256];
   __shared__ int s_max[EV_WARPS], s_ties[EV_WARPS], s_holes[EV_WARPS], s_movers[EV_WARPS], warp_tot[8];
@@ -126,9 +126,9 @@ evict_select_kernel(EvArgs A, int held) {
   }
   // the latest position
   int latest = -0x7fffffff;
-  for (int j = e0 + tid; j < e1; j += 4 * EV_THREADS) {
+  for (int j = e0 + tid; j < e1; j += AHEAD * EV_THREADS) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       if (j + i * EV_THREADS < e1) latest = max(latest, P[j + i * EV_THREADS]);
   }
   latest = __reduce_max_sync(0xffffffffu, latest);
@@ -154,14 +154,14 @@ evict_select_kernel(EvArgs A, int held) {
     const int shift = 24 - 8 * pass;
     int* const hs = hist[pass & 1];
     if (pass == 0) {
-      for (int j = e0 + tid; j < e1; j += 4 * EV_THREADS) {
-        int p[4];
-        float w[4];
+      for (int j = e0 + tid; j < e1; j += AHEAD * EV_THREADS) {
+        int p[AHEAD];
+        float w[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < AHEAD; ++i)
           if (j + i * EV_THREADS < e1) { p[i] = P[j + i * EV_THREADS]; w[i] = W[j + i * EV_THREADS]; }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < AHEAD; ++i)
           if (j + i * EV_THREADS < e1) {
             const unsigned key = key_of(p[i], w[i]);
             if (held) keys[j + i * EV_THREADS - e0] = key;
@@ -267,14 +267,14 @@ evict_select_kernel(EvArgs A, int held) {
   if (rank == 0 && tid == 0) moves[0] = all_movers;
   // The kept entries that do not move, where the outputs are other tensors: on their way while the lists are written.
   if (held && Wo != W) {
-    for (int j = e0 + tid; j < min(e1, keep); j += 4 * EV_THREADS) {
-      float w[4];
-      int p[4];
+    for (int j = e0 + tid; j < min(e1, keep); j += AHEAD * EV_THREADS) {
+      float w[AHEAD];
+      int p[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < AHEAD; ++i)
         if (j + i * EV_THREADS < min(e1, keep)) { w[i] = W[j + i * EV_THREADS]; p[i] = P[j + i * EV_THREADS]; }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < AHEAD; ++i) {
         const int at = j + i * EV_THREADS;
         if (at < min(e1, keep) && ((bits[(at - e0) >> 5] >> ((at - e0) & 31)) & 1u)) {
           Wo[at] = w[i];
