@@ -617,3 +617,66 @@ def test_accumulate_attention_of_requests_without_tokens(dtype):
         c = _weights_case(dtype, 4, 2, 64, 16, q_lens, ctx_lens, 95)
         c["qkv"] = c["qkv"] if sum(q_lens) else torch.zeros(0, 8 * 64, dtype=dtype)
         _check_weights(c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_lens,ctx_lens", [([1, 1], [700, 20]), ([2], [5000]), ([40], [30])])
+def test_accumulate_attention_over_wide_latents(dtype, q_lens, ctx_lens):
+    """Heads of 576 channels over one plane and one kv head: beyond what the tensor cores' tiles take for many rows."""
+    _check_weights(_weights_case(dtype, 16, 1, 576, 16, q_lens, ctx_lens, 97, planes=1, std=0.3))
+
+
+def test_with_the_steps_arena():
+    """Scratch memory from a step's arena, too small at first (it falls back, grows at the reset) and then of the right size: the same bits."""
+    from qwen_engine_b200.parts.base import Arena
+    arena = Arena(DEV, capacity=1 << 12)
+    for q_lens, ctx_lens in (([1, 2], [700, 5000]), ([150], [40])):
+        c = _weights_case(torch.bfloat16, 8, 2, 128, 16, q_lens, ctx_lens, 98)
+        want = _gather(c)[0]
+        Hq, Hkv, D = c["heads"]
+        for _ in range(3):
+            arena.reset()
+            w = c["weights"].to(DEV)
+            out = torch.full_like(w, -5.0)
+            ops.accumulate_attention(c["qkv"].to(DEV), c["pages"].to(DEV), c["table"].to(DEV), _context(c), w, out, D ** -0.5, 0, Hq, Hkv, D, arena.alloc)
+            assert torch.equal(out.cpu(), want)
+    v = _verify_case(3, [2], 501, 16, True)
+    want = plain_drafts.verify(**v)
+    d = {k: x.to(DEV) for k, x in v.items()}
+    for _ in range(2):
+        arena.reset()
+        tokens, counts = torch.zeros(9, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+        ops.verify_drafts(d["logits"], d["draft_tokens"], d["draft_logits"], d["row_starts"], d["temperature"], d["top_k"], d["uniform"], tokens, counts, arena.alloc)
+        _same((tokens.cpu(), counts.cpu()), want)
+
+
+def test_drafts_through_the_step_function():
+    """A model's own step with a request's newest token and its drafts, every place wanted: greedy requests gain exactly the tokens that decoding one by
+    one gives, drafts that stand and the first that does not."""
+    from qwen_engine_b200.cache.manager import CacheManager
+    from qwen_engine_b200.config import preset_config_dict
+    from qwen_engine_b200.engine.loading import load_model
+    from qwen_engine_b200.engine.runner import StepEntry
+    from qwen_engine_b200.registry import config_from_dict
+    loaded = load_model(None, torch.float32, DEV, 16, 64, 4, False, config=config_from_dict(preset_config_dict("tiny-b")), random_seed=3)
+    runner, cache = loaded.runner, loaded.cache
+    assert isinstance(cache, CacheManager)
+    prompt = [5, 6, 7, 8, 9]
+    rc = cache.open("one by one")
+    logits = runner.step([StepEntry(rc, prompt, [len(prompt) - 1])])
+    truth = [int(logits[0].argmax())]
+    for _ in range(4):
+        logits = runner.step([StepEntry(rc, [truth[-1]], [0])])
+        truth.append(int(logits[0].argmax()))
+    cache.close(rc)
+    greedy = [SamplingParams(temperature=0.0)]
+    for wrong in (None, 0, 2):
+        drafts = list(truth[1:4])
+        if wrong is not None:
+            drafts[wrong] = (drafts[wrong] + 1) % 389
+        rc = cache.open(f"drafted {wrong}")
+        runner.step([StepEntry(rc, prompt, [len(prompt) - 1])])
+        logits = runner.step([StepEntry(rc, [truth[0]] + drafts, range(4))])
+        got = Sampler(DEV).verify(logits, greedy, [drafts], [[0.5] * 4])
+        assert got == [truth[1:5] if wrong is None else truth[1:wrong + 2]]
+        cache.close(rc)
