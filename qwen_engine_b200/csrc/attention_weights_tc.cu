@@ -17,7 +17,8 @@
 // all that it delivers; measured, with the readers beside it, about 950), its 16 384 exponentials the special-function unit 1 024, and the
 // readers' instructions their issue slots about as long.  An eighth of the exponentials is a polynomial (at2_poly2), two at a time on the float32
 // units: none 256, an eighth 249, a quarter 259, three eighths 271 us for a prompt of 4 096 tokens with 32 / 8 heads (one CTA walking several
-// units 269: some are empty, and they are dealt out beforehand).
+// units 269: some are empty, and they are dealt out beforehand; 128 x 256 products in two accumulators 258).  With all heads' longest units first and
+// a unit an SM instead of four: 217.
 //
 // Every wait is bounded: one that runs out records a code, raises the CTA's abort flag, and the CTA leaves without writing.
 #include "attention_weights.cuh"
@@ -179,7 +180,7 @@ attention_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   extern __shared__ unsigned char raw[];
   AwTcSmem& sm = *reinterpret_cast<AwTcSmem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int c = blockIdx.y, r = blockIdx.z, part = blockIdx.x % C.parts, G = A.Hq / A.Hkv, tpt = C.tpt;
+  const int c = blockIdx.x / C.parts % A.Hkv, r = blockIdx.z, part = blockIdx.x % C.parts, G = A.Hq / A.Hkv, tpt = C.tpt;
   pdl_launch_dependents();
   pdl_wait();                                     // (lengths and counts are an earlier kernel's)
   const AwReq R = aw_req(A, r);
@@ -188,8 +189,9 @@ attention_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   // the unit's A tiles a0 .. a0 + n_a - 1, and its part b0 .. b1 - 1 of the B tiles that meet them
   int a0, n_a, b0, b1;
   {
-    const int groups = gridDim.x / C.parts, order = blockIdx.x / C.parts;
-    const int group = PASS == 1 ? groups - 1 - order : order;                     // (the longest units first)
+    // the longest units first, all heads' before the next: CTAs start in this order, and what starts last is short
+    const int groups = gridDim.x / (C.parts * A.Hkv), order = blockIdx.x / (C.parts * A.Hkv);
+    const int group = PASS == 1 ? groups - 1 - order : order;
     a0 = group * C.na;
     if (PASS == 1) {
       const int nq = (R.counted + tpt - 1) / tpt;
@@ -514,7 +516,7 @@ extern "C" int qe_attention_weights_tc(const void* q, long q_stride, int T, cons
     if (!qe_tensor_map_bf16(pages, 5, dims, strides, box, &map_k)) return 1;
   }
   const int q_tiles = (max_q + C.tpt - 1) / C.tpt, k_tiles = (max_total + AT2_TILE - 1) / AT2_TILE;
-  const dim3 grid1((unsigned)((q_tiles + C.na - 1) / C.na * parts1), (unsigned)Hkv, (unsigned)R), grid2((unsigned)((k_tiles + C.na - 1) / C.na * parts2), (unsigned)Hkv, (unsigned)R);
+  const dim3 grid1((unsigned)((q_tiles + C.na - 1) / C.na * parts1 * Hkv), 1, (unsigned)R), grid2((unsigned)((k_tiles + C.na - 1) / C.na * parts2 * Hkv), 1, (unsigned)R);
   const bool general = softcap > 0.f || slopes != nullptr;
   C.parts = parts1;
   cudaError_t e = general ? at2_launch<1, true>(grid1, stream, map_q, map_k, A, C) : at2_launch<1, false>(grid1, stream, map_q, map_k, A, C);

@@ -1745,8 +1745,9 @@ ATTENTION_WEIGHTS_TC = True                   # more rows in bfloat16: the kerne
 
 
 def attention_weights_tc_parts(units: int, tiles: int) -> int:
-    """In how many parts each unit's walk over ``tiles`` tiles is cut: four units an SM, four tiles a part at least."""
-    return max(1, min(-(-4 * TC_TARGET_CTAS // max(1, units)), -(-tiles // 4), ATTENTION_WEIGHTS_MAX_PARTS))
+    """In how many parts each unit's walk over ``tiles`` tiles is cut: a unit an SM (with four: a prompt of 4 096 tokens, 32 / 8 heads,
+    239 us for 217, 64 tokens behind 32 000 112 for 95), four tiles a part at least."""
+    return max(1, min(-(-TC_TARGET_CTAS // max(1, units)), -(-tiles // 4), ATTENTION_WEIGHTS_MAX_PARTS))
 
 
 def _cluster_smem(rows: int, head_dim: int, part: int) -> int:
@@ -1770,7 +1771,9 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
     the others' keys get no weight.
     ``window``, ``slopes``, ``softcap``, ``sinks``: as in ``paged_attention``.  Keys that lie in no page get no weight; distances
     are of places in the cache, so that a window or a distance bias goes with a cache that nothing was evicted from.
-    ``alloc(shape, dtype)`` gives scratch memory.  Float32 sums in one order: equal calls give equal bits."""
+    ``alloc(shape, dtype)`` gives scratch memory.  Float32 sums in one order: equal calls give equal bits.  Launches go by the
+    requests' tokens (ctx.q_lens_host): a captured call may be replayed with other cached lengths, pages, slots and ``counted``
+    on the device, not with other numbers of tokens."""
     Hq, Hkv, D = num_heads, num_kv_heads, head_dim
     T, R, planes = qkv.shape[0], int(ctx.num_reqs), int(kv_pages.shape[1]) if kv_pages.dim() == 5 else 0
     _rows(qkv, "accumulate_attention: qkv")
