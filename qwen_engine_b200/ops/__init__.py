@@ -1858,13 +1858,14 @@ def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torc
     into the places before it that come free, in theirs; the others do not move, so the order of a cache's keys is not kept
     (attention without a window or a distance bias does not look at it; ``positions`` say which token is where).
 
-    cache: a group's tensor [layers, pages, planes, Hkv, page, D], all planes of an entry move; block_tables int32 [R, blocks];
+    cache: a group's tensor [layers, pages, planes, Hkv, page, D] (two bytes an element or a multiple), all planes of an entry move; block_tables int32 [R, blocks];
     slot_ids int32 [R]: the rows of ``weights`` (float32) and ``positions`` (int32), both [layers, slots, Hkv, capacity], that
     belong to the requests; lens int32 [R] on the device.  weights_out and positions_out get the kept entries' weights and
     positions in their new places (places from min(lens, keep) on stay as they are); they may be the inputs themselves.
     A request's positions are distinct, pages it moves within are its own (not shared with another request), no two requests
     have one slot.  ``alloc(shape, dtype)`` gives scratch memory."""
-    _need(cache.dim() == 6 and cache.is_contiguous(), "evict_tokens: cache must be contiguous [layers, pages, planes, Hkv, page, D]")
+    _need(cache.dim() == 6 and cache.is_contiguous() and cache.element_size() % 2 == 0,
+          "evict_tokens: cache must be contiguous [layers, pages, planes, Hkv, page, D], of two bytes an element or a multiple")
     S, pages, planes, Hkv, page, D = (int(n) for n in cache.shape)
     _i32(block_tables, "block_tables")
     _i32(slot_ids, "slot_ids")

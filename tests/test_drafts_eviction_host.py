@@ -82,7 +82,8 @@ def _evict_args(**other):
 
 
 @pytest.mark.parametrize("other", [
-    dict(cache=torch.zeros(6, 2, 2, 8, 16)), dict(cache=torch.zeros(2, 6, 2, 2, 16, 8).transpose(4, 5)), dict(block_tables=torch.zeros(3, 2, dtype=torch.int32)),
+    dict(cache=torch.zeros(6, 2, 2, 8, 16)), dict(cache=torch.zeros(2, 6, 2, 2, 16, 8).transpose(4, 5)),
+    dict(cache=torch.zeros(2, 6, 2, 2, 8, 15, dtype=torch.uint8)), dict(block_tables=torch.zeros(3, 2, dtype=torch.int32)),
     dict(slot_ids=torch.zeros(3, dtype=torch.int32)), dict(lens=torch.zeros(2)), dict(weights=torch.zeros(1, 3, 2, 16)),
     dict(weights=torch.zeros(2, 3, 2, 16, dtype=torch.bfloat16)), dict(positions=torch.zeros(2, 3, 2, 17, dtype=torch.int32)),
     dict(weights_out=torch.zeros(2, 3, 2, 17)), dict(positions_out=torch.zeros(2, 3, 2, 16)), dict(keep=0), dict(first=-1), dict(recent=-1),
