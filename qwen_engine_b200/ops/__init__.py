@@ -1828,7 +1828,7 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
             None if scores is None else scores.data_ptr(), ld, stream), "accumulate_attention")
         if few >= max_q * G:
             return
-    if (ATTENTION_WEIGHTS_TC and qkv.dtype == torch.bfloat16 and pq % 16 == 0 and qkv.stride(0) % 8 == 0 and pk % 16 == 0 and max_q > 0
+    if (ATTENTION_WEIGHTS_TC and qkv.dtype == torch.bfloat16 and pq % 16 == 0 and qkv.stride(0) % 8 == 0 and qkv.stride(0) > 0 and pk % 16 == 0 and max_q > 0
             and lib().qe_attention_weights_tc_supported(Hq, Hkv, D, page)):
         tpt, na = 128 // G, 4 if D <= 128 else (2 if D <= 192 else 1)      # tokens of a tile of queries, tiles a unit
         many = [(n, n + c) for n, c in zip(ctx.q_lens_host, ctx.ctx_lens_host) if n * G > few]

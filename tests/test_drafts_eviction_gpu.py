@@ -680,3 +680,17 @@ def test_drafts_through_the_step_function():
         got = Sampler(DEV).verify(logits, greedy, [drafts], [[0.5] * 4])
         assert got == [truth[1:5] if wrong is None else truth[1:wrong + 2]]
         cache.close(rc)
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 40), (torch.bfloat16, 3), (torch.bfloat16, 70)])
+def test_rows_that_are_one_row_in_memory(dtype, n):
+    """A row given n times over by a stride of 0 gathers what n equal rows gather."""
+    c = _weights_case(dtype, 8, 2, 128, 16, [n], [50], 23)
+    c["qkv"] = c["qkv"][:1].repeat(n, 1)
+    Hq, Hkv, D = c["heads"]
+    w = c["weights"].to(DEV)
+    out = w.clone()
+    ops.accumulate_attention(c["qkv"][:1].to(DEV).expand(n, -1), c["pages"].to(DEV), c["table"].to(DEV), _context(c), w, out, D ** -0.5, 0, Hq, Hkv, D, _alloc)
+    want, tol = plain_drafts.gathered(c["qkv"], c["pages"], c["table"], c["cu"], c["ctx"], c["slots"], c["weights"], c["weights"],
+                                      D ** -0.5, 0, Hq, Hkv, D, None)
+    assert ((out.cpu().double() - want).abs() <= tol).all()
