@@ -463,12 +463,12 @@ verify_draw_kernel(const float* __restrict__ logits, const float* __restrict__ d
         stands = vf_argmax(parts, lo + i, chunks) == d;
       } else {
         const VfStat sp = vf_stat(parts, lo + i, chunks, c);
-        const float x = logits[(size_t)(lo + i) * V + d];
+        const float x = fmaxf(logits[(size_t)(lo + i) * V + d], -INFINITY);                 // (NaN as -inf)
         const double p = vf_key(x) >= thresholds[lo + i] ? (x == sp.m ? 1.0 : (double)vf_ex2((x - sp.m) * c)) : 0.0;
         double q = 1.0, zq = 1.0;
         if (draft_logits) {
           const VfStat sq = vf_stat(parts, N + d0 + i, chunks, c);
-          const float xd = draft_logits[(size_t)(d0 + i) * V + d];
+          const float xd = fmaxf(draft_logits[(size_t)(d0 + i) * V + d], -INFINITY);
           q = vf_key(xd) >= thresholds[N + d0 + i] ? (xd == sq.m ? 1.0 : (double)vf_ex2((xd - sq.m) * c)) : 0.0;
           zq = sq.z;
         }

@@ -694,3 +694,15 @@ def test_rows_that_are_one_row_in_memory(dtype, n):
     want, tol = plain_drafts.gathered(c["qkv"], c["pages"], c["table"], c["cu"], c["ctx"], c["slots"], c["weights"], c["weights"],
                                       D ** -0.5, 0, Hq, Hkv, D, None)
     assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+# ---- rows with little or nothing in them -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("V", [97, 4099, 40001])
+def test_verify_drafts_whose_own_draft_logit_is_nan(V):
+    """A NaN counts as -inf: the draft's probability is 0, and so it stands wherever the target gives it any."""
+    for top_k in (0, 5):
+        c = _verify_case(12, [1, 3], V, 500 + top_k, True, top_ks=(top_k,), temps=(0.7, 1.3))
+        for j, d in enumerate(c["draft_tokens"].tolist()):
+            c["draft_logits"][j, d] = math.nan if j % 2 else -math.inf
+        _same(_verify(c), plain_drafts.verify(**c))
