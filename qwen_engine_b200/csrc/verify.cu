@@ -394,6 +394,7 @@ __device__ __forceinline__ VfStat vf_stat(const VfPart* parts, size_t y, int chu
   for (int o = 0; o < VF_MAX_CTAS; ++o) s.z += z[o] * (m[o] == s.m ? 1.0 : (double)vf_ex2((m[o] - s.m) * c));
   return s;
 }
+// the lowest place of a row's largest logit, -1 where none is above -inf
 __device__ __forceinline__ int vf_argmax(const VfPart* parts, size_t y, int chunks) {
   float m = -INFINITY;
   int at = 0x7fffffff;
@@ -401,7 +402,7 @@ __device__ __forceinline__ int vf_argmax(const VfPart* parts, size_t y, int chun
     const VfPart p = parts[y * chunks + o];
     if (p.m > m) { m = p.m; at = p.arg; }
   }
-  return at == 0x7fffffff ? 0 : at;
+  return at == 0x7fffffff ? -1 : at;
 }
 // exp((x - m) / T) in float64, x <= m finite: with y = 32 log2(e) (x - m) / T = 32 i + j + f, 2^i 2^(j / 32) (1 + f' + f'^2 / 2 + f'^3 / 6 + f'^4 / 24),
 // f' = f ln 2 / 32.  The first term left out is below (ln 2 / 64)^5 / 120 = 1.3 10^-12.  k = 32 log2(e) / T; `pow` holds 2^(j / 32).
@@ -485,7 +486,7 @@ verify_draw_kernel(const float* __restrict__ logits, const float* __restrict__ d
     if (tid == 0) counts[r] = a + 1;
   }
   if (greedy) {
-    if (rank == 0 && tid == 0) tokens[lo + a] = vf_argmax(parts, lo + a, chunks);
+    if (rank == 0 && tid == 0) tokens[lo + a] = max(vf_argmax(parts, lo + a, chunks), 0);
     return;
   }
   const VfRow P(logits + (size_t)(lo + a) * V, V);

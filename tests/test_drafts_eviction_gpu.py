@@ -706,3 +706,20 @@ def test_verify_drafts_whose_own_draft_logit_is_nan(V):
         for j, d in enumerate(c["draft_tokens"].tolist()):
             c["draft_logits"][j, d] = math.nan if j % 2 else -math.inf
         _same(_verify(c), plain_drafts.verify(**c))
+
+
+@pytest.mark.parametrize("model", [True, False])
+@pytest.mark.parametrize("V", [5, 333, 9001])
+def test_verify_drafts_of_token_0_where_a_greedy_row_has_nothing(V, model):
+    """A row without any logit above -inf lets no draft stand, not the draft of token 0 either, and gives token 0."""
+    c = _verify_case(8, [1, 3], V, 600 + V, model, temps=(0.0, 0.0, 0.8))
+    starts = c["row_starts"].tolist()
+    c["draft_tokens"][:] = c["logits"][[starts[r] + i for r in range(8) for i in range(starts[r + 1] - starts[r] - 1)]].argmax(1).to(torch.int32)
+    for r in range(8):
+        row = starts[r] + (r % 2) * (starts[r + 1] - starts[r] - 2)              # the request's first or last drafted place
+        c["logits"][row] = math.nan if r % 3 == 0 else -math.inf
+        c["draft_tokens"][row - r] = 0
+    want = plain_drafts.verify(**c)
+    for r in range(8):
+        assert int(want[1][r]) <= 1 + (r % 2) * (starts[r + 1] - starts[r] - 2)
+    _same(_verify(c), want)
