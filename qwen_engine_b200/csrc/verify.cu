@@ -14,8 +14,9 @@
 //
 // The top_k-th largest logit.  Of a chunk's logits only the k largest can be among the row's k largest, and the k-th largest of
 // the threads' maxima (of the maxima of either half of their logits, for a k of some hundreds) is a lower bound of the chunk's k-th largest: hardly
-// more than k logits reach it.  The CTAs list theirs, and the k-th largest of the lists (each number compared with every other, or bit by bit) is the
-// row's.  Where k is large, or the lists overflow (equal logits), the digits of an order-preserving integer are found one
+// more than k logits reach it.  (A thread without a logit above -inf counts with the lowest finite number, so the bound is one of the logits above
+// -inf; where fewer than k of those are listed, they are all that the row has, and all are kept.)  The CTAs list theirs, and the k-th largest of the
+// lists (each number compared with every other, or bit by bit) is the row's.  Where k is large, or the lists overflow (equal logits), the digits of an order-preserving integer are found one
 // after the other from histograms that meet in distributed shared memory.
 //
 // Precision.  Whether a draft stands is one comparison of float32 exponentials with float64 sums: it goes the other way
@@ -225,8 +226,8 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
     bool from_list = false;
     const int kc = (k + C - 1) / C;
     if (kc <= VF_LIST_K) {
-      // The high half of the k / C-th largest of the threads' maxima, in every chunk: at least k logits reach the least of those
-      // numbers, so it is a lower bound of the row's k-th largest.
+      // The high half of the k / C-th largest of the threads' maxima, in every chunk: at least k logits, or all above -inf, reach the
+      // least of those numbers, so it is a lower bound of the k-th largest of the logits above -inf.
       unsigned low = 0u;
       const unsigned h0 = vf_key(half[0]), h1 = g0 + tid + VF_THREADS < g1 ? vf_key(half[1]) : 0u;
       for (int bit = 31; bit >= 16; --bit) {
@@ -274,7 +275,9 @@ verify_sums_kernel(const float* __restrict__ logits, const float* __restrict__ d
       if (from_list && tid < 4) all[total + tid] = 0u;         // (read four at a time below)
       cluster_sync_all();                       // the lists have been read
       if (from_list) {
-        if (total <= VF_RANKED) {
+        if (total < (unsigned)k) {
+          thr = 0u;                             // all that is above -inf is listed, and stays
+        } else if (total <= VF_RANKED) {
           // the k-th largest: the one with fewer than k above it and at least k with its equals
           if (tid < total) {
             const unsigned key = all[tid];

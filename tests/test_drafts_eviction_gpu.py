@@ -723,3 +723,36 @@ def test_verify_drafts_of_token_0_where_a_greedy_row_has_nothing(V, model):
     for r in range(8):
         assert int(want[1][r]) <= 1 + (r % 2) * (starts[r + 1] - starts[r] - 2)
     _same(_verify(c), want)
+
+
+@pytest.mark.parametrize("top_k", [3, 50, 1000])
+@pytest.mark.parametrize("V", [333, 4099, 32003, 151936])
+def test_verify_drafts_with_fewer_finite_logits_than_top_k(V, top_k):
+    """Rows of which 1 to top_k - 1 logits are above -inf (all of those are kept), of the target's and of the draft model's, among rows that are whole:
+    nothing of one row's top_k-th logit shows in another's, and equal calls give equal tokens."""
+    rnd = random.Random(V + top_k)
+    for seed, model in ((0, True), (1, True), (2, False)):
+        c = _verify_case(7, [2, 4], V, 400 + seed, model, top_ks=(0, top_k, top_k), temps=(0.6, 1.0))
+        starts = c["row_starts"].tolist()
+        draft_of = {starts[r] + i: starts[r] + i - r for r in range(7) for i in range(starts[r + 1] - starts[r] - 1)}      # row -> draft
+
+        def thin(x, draft):
+            """All but a few of the row's logits go; the draft's own mostly stays."""
+            n = rnd.randint(1, min(top_k, V) - 1)
+            stay = rnd.sample(range(V), n)
+            if draft is not None and rnd.random() < 0.8:
+                stay[0] = int(c["draft_tokens"][draft])
+            kept = x[stay].clone()
+            x[:] = -math.inf
+            x[::5] = math.nan
+            x[stay] = kept
+        for row in range(c["logits"].shape[0]):
+            if row % 3 != 2:
+                thin(c["logits"][row], draft_of.get(row))
+        if model:
+            for j in range(c["draft_logits"].shape[0]):
+                if j % 3 != 1:
+                    thin(c["draft_logits"][j], j)
+        got = _verify(c)
+        _same(got, plain_drafts.verify(**c))
+        _same(_verify(c), got)
