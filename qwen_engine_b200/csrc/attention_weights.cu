@@ -162,10 +162,10 @@ attention_weights_rows_kernel(AwArgs A, int few_rows) {
         s[i][j] = seen ? aw_score(A, s[i][j], slope, pos - key) : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
-      if (mx == -INFINITY) continue;
-      float sum = z[i] * exp2f(m[i] - mx);
+      const float base = aw_base(mx);
+      float sum = z[i] * exp2f(m[i] - base);
 #pragma unroll
-      for (int j = 0; j < KM; ++j) sum += exp2f(s[i][j] - mx);
+      for (int j = 0; j < KM; ++j) sum += exp2f(s[i][j] - base);
       m[i] = mx; z[i] = sum;
     }
   }
@@ -175,8 +175,8 @@ attention_weights_rows_kernel(AwArgs A, int few_rows) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m[i], o), oz = __shfl_xor_sync(0xffffffffu, z[i], o);
-      const float nm = fmaxf(m[i], om);
-      if (nm != -INFINITY) z[i] = z[i] * exp2f(m[i] - nm) + oz * exp2f(om - nm);
+      const float nm = fmaxf(m[i], om), base = aw_base(nm);
+      z[i] = z[i] * exp2f(m[i] - base) + oz * exp2f(om - base);
       m[i] = nm;
     }
     const int rho = rho0 + aw_own<RM>(ty, i);

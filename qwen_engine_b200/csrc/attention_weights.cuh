@@ -61,12 +61,18 @@ __device__ __forceinline__ int aw_page(const AwArgs& A, int r, int key) {
   return p < A.num_pages ? p : -1;
 }
 
-// A row's parts put together: the maximum, and the reciprocal of the softmax's denominator (0 for a row that sees nothing).
+// A row's maximum as exponents are taken relative to it: 0 where there is none (a row that sees nothing, or nothing but -inf and NaN), so that
+// what is added up is 0, or NaN for a NaN.
+__device__ __forceinline__ float aw_base(float m) { return m == -INFINITY ? 0.f : m; }
+
+// A row's parts put together: the maximum, and the reciprocal of the softmax's denominator (0 for a row that sees nothing, NaN for one
+// that sees a NaN).
 __device__ __forceinline__ float2 aw_merge(const float* st, int parts, const float* sink) {
   float m = -INFINITY, z = 0.f;
   for (int p = 0; p < parts; ++p) m = fmaxf(m, st[2 * p]);
-  if (m == -INFINITY) return make_float2(0.f, 0.f);
-  for (int p = 0; p < parts; ++p) z += st[2 * p + 1] * exp2f(st[2 * p] - m);
+  const float base = aw_base(m);
+  for (int p = 0; p < parts; ++p) z += st[2 * p + 1] * exp2f(st[2 * p] - base);
+  if (m == -INFINITY) return make_float2(0.f, z);       // (0 or NaN)
   if (sink) z += exp2f(*sink * AW_LOG2E - m);
   return make_float2(m, 1.f / z);
 }

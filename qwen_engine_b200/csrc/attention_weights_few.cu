@@ -204,8 +204,8 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
 #pragma unroll
       for (int o = 1; o <= 2; o <<= 1) {
         const float om = __shfl_xor_sync(0xffffffffu, m[mt][h], o), oz = __shfl_xor_sync(0xffffffffu, z[mt][h], o);
-        const float nm = fmaxf(m[mt][h], om);
-        if (nm != -INFINITY) z[mt][h] = z[mt][h] * aw_ex2(m[mt][h] - nm) + oz * aw_ex2(om - nm);
+        const float nm = fmaxf(m[mt][h], om), base = aw_base(nm);
+        z[mt][h] = z[mt][h] * aw_ex2(m[mt][h] - base) + oz * aw_ex2(om - base);
         m[mt][h] = nm;
       }
       if (x == 0) { warp_ml[warp][mt * 16 + 8 * h + n][0] = m[mt][h]; warp_ml[warp][mt * 16 + 8 * h + n][1] = z[mt][h]; }
@@ -215,9 +215,9 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
     float mm = -INFINITY, zz = 0.f;
 #pragma unroll
     for (int w = 0; w < AF_WARPS; ++w) mm = fmaxf(mm, warp_ml[w][tid][0]);
-    if (mm != -INFINITY)
+    const float base = aw_base(mm);
 #pragma unroll
-      for (int w = 0; w < AF_WARPS; ++w) zz += warp_ml[w][tid][1] * aw_ex2(warp_ml[w][tid][0] - mm);
+    for (int w = 0; w < AF_WARPS; ++w) zz += warp_ml[w][tid][1] * aw_ex2(warp_ml[w][tid][0] - base);
     row_max[tid] = mm;
     row_sum[tid] = zz;
   }
@@ -261,13 +261,14 @@ attention_weights_cluster_kernel(AwArgs A, int max_rows, int part_keys) {
     float m = -INFINITY, z = 0.f;
     for (int o = 0; o < C; ++o) m = fmaxf(m, cluster_ld_f32(cluster_map_shared(&row_max[tid], o)));
     float2 v = make_float2(0.f, 0.f);
-    if (tid < rows && m != -INFINITY) {
+    if (tid < rows) {
+      const float base = aw_base(m);
       for (int o = 0; o < C; ++o) {
         const float om = cluster_ld_f32(cluster_map_shared(&row_max[tid], o));
-        z += cluster_ld_f32(cluster_map_shared(&row_sum[tid], o)) * exp2f(om - m);
+        z += cluster_ld_f32(cluster_map_shared(&row_sum[tid], o)) * exp2f(om - base);
       }
-      if (A.sinks) z += exp2f(A.sinks[c * G + tid % G] * AW_LOG2E - m);
-      v = make_float2(m, 1.f / z);
+      if (A.sinks) z += exp2f(A.sinks[c * G + tid % G] * AW_LOG2E - base);
+      v = m == -INFINITY ? make_float2(0.f, z == z ? 0.f : z) : make_float2(m, 1.f / z);
     }
     row[tid] = v;
   }

@@ -68,6 +68,13 @@ __device__ __forceinline__ float2 at2_add(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+__device__ __forceinline__ float2 at2_mul(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float at2_max_nan(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b)); return d; }
 __device__ __forceinline__ float at2_max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
 // waits for the loads from tensor memory; the registers are operands, so that nothing that reads them is moved in front of it
@@ -81,9 +88,10 @@ __device__ __forceinline__ void at2_wait_ld(uint32_t (&u)[32]) {
 __device__ __forceinline__ int at2_tile0(const AwReq& R, int r, int tpt) { return R.row0 / tpt + r; }
 
 // 2^x of two x <= 0 (or a little above) without the special-function unit: x = n + f, |f| <= 1/2, 2^f by a polynomial of degree 5 that is 1 at 0 and
-// whose largest relative error on the interval is least (fitted by weighted least squares; 1.6 10^-7 with its float32 coefficients), n into the exponent.
+// whose largest relative error on the interval is least (fitted by weighted least squares; 1.6 10^-7 with its float32 coefficients), times 2^n.
+// NaN stays NaN: a weight must not depend on which columns come here.
 __device__ __forceinline__ float2 at2_poly2(float2 x) {
-  x.x = fmaxf(x.x, -127.f); x.y = fmaxf(x.y, -127.f);           // (there n = -127 and f = 0 give the bits of 0; between that and -126.5 f > 0 gives a subnormal)
+  x.x = at2_max_nan(x.x, -127.f); x.y = at2_max_nan(x.y, -127.f);         // (2^-127 counts as 0)
   const float magic = 12582912.f;                              // 1.5 2^23: the sum's low bits are x rounded to an integer
   const float2 t = at2_add(x, make_float2(magic, magic)), n = at2_add(t, make_float2(-magic, -magic));
   const float2 f = at2_fma(n, make_float2(-1.f, -1.f), x);
@@ -93,7 +101,8 @@ __device__ __forceinline__ float2 at2_poly2(float2 x) {
   p = at2_fma(p, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
   p = at2_fma(p, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
   p = at2_fma(p, f, make_float2(1.f, 1.f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  // 2^n as a factor, which a NaN survives
+  return at2_mul(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 // whether the pair of columns 2 j, 2 j + 1 of a chunk goes there
 __device__ constexpr bool at2_on_poly(int j) { return (j & 7) == 1; }
@@ -388,8 +397,8 @@ attention_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         for (int o = w + n_seq; o < AT2_GROUPS; o += n_seq) {
           const float2 v = sm.meet[o][rr];
           if (PASS == 1) {
-            const float m = fmaxf(row.m, v.x);
-            if (m != -INFINITY) row.z = row.z * exp2f(row.m - m) + v.y * exp2f(v.x - m);
+            const float m = fmaxf(row.m, v.x), base = aw_base(m);
+            row.z = row.z * exp2f(row.m - base) + v.y * exp2f(v.x - base);
             row.m = m;
           } else {
             total += v.x;
@@ -436,7 +445,7 @@ attention_weights_merge_kernel(AwArgs A, AwTc C) {
   if (rr < C.tpt * G && t < R.counted) {
     const int head = c * G + rr % G;
     const float2 mz = aw_merge(A.stats + ((size_t)(R.row0 + t) * A.Hq + head) * C.parts * 2, C.parts, A.sinks ? A.sinks + head : nullptr);
-    if (mz.y > 0.f) v = log2f(mz.y) - mz.x;         // (a row that sees nothing gives nothing)
+    if (mz.y != 0.f) v = log2f(mz.y) - mz.x;        // (a row that sees nothing gives nothing, one that sees a NaN gives NaN)
   }
   C.negl[((size_t)c * C.tiles + at2_tile0(R, r, C.tpt) + tile) * AT2_TILE + rr] = v;
 }

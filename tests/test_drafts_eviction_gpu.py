@@ -756,3 +756,65 @@ def test_verify_drafts_with_fewer_finite_logits_than_top_k(V, top_k):
         got = _verify(c)
         _same(got, plain_drafts.verify(**c))
         _same(_verify(c), got)
+
+
+# ---- NaN in what a row sees ----------------------------------------------------------------------------------------------------------
+
+NAN_BATCHES = [(torch.float32, [2, 3], [70, 9], {}), (torch.bfloat16, [2, 3], [70, 9], {}), (torch.bfloat16, [3, 2], [5000, 40], {}),
+               (torch.bfloat16, [150, 40], [40, 7], {}), (torch.bfloat16, [150, 40], [40, 7], {"tc": False}), (torch.bfloat16, [150, 40], [40, 7], {"softcap": 3.0}),
+               (torch.bfloat16, [90, 40], [300, 7], {"window": 100}), (torch.float32, [90, 40], [300, 7], {"window": 100})]
+
+
+def _check_nan(c, clean, row, head, seen, monkeypatch, options):
+    """Request 0's kv head of ``head``: the keys ``seen`` are NaN.  Every other head and request: as without the NaN."""
+    Hq, Hkv, D = c["heads"]
+    opts = dict(options)
+    monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_TC", opts.pop("tc", True))
+    got, _ = _gather(c, opts.pop("window", 0), **opts)
+    kv, s0 = head // (Hq // Hkv), int(c["slots"][0])
+    assert torch.isnan(got[s0, kv, :len(seen)][seen]).all(), (row, head, (~torch.isnan(got[s0, kv, :len(seen)]) & seen).nonzero().flatten().tolist()[:5])
+    other = torch.ones(got.shape, dtype=torch.bool)
+    other[s0, kv, :len(seen)] = False
+    assert torch.equal(got[other], clean[other])
+
+
+@pytest.mark.parametrize("dtype,q_lens,ctx_lens,options", NAN_BATCHES)
+def test_accumulate_attention_of_a_query_that_is_nan(dtype, q_lens, ctx_lens, options, monkeypatch):
+    """Every key that the row sees becomes NaN, whatever the row's place in its tile and whichever kernel serves."""
+    Hq, Hkv, D = 4, 2, 128
+    c = _weights_case(dtype, Hq, Hkv, D, 16, q_lens, ctx_lens, 700)
+    window = options.get("window", 0)
+    clean = _gather(c, window, **{k: v for k, v in options.items() if k == "softcap"})[0] if options.get("tc", True) else None
+    if clean is None:
+        monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_TC", False)
+        clean = _gather(c)[0]
+    total = q_lens[0] + ctx_lens[0]
+    key = torch.arange(total)
+    for row in range(0, q_lens[0], 1 if q_lens[0] < 8 else 9):
+        for head in (0, 1, 3):
+            d = dict(c, qkv=c["qkv"].clone())
+            d["qkv"][row, head * D + 5] = math.nan
+            pos = ctx_lens[0] + row
+            seen = (key <= pos) & ((key > pos - window) if window else torch.ones(total, dtype=torch.bool))
+            _check_nan(d, clean, row, head, seen, monkeypatch, options)
+
+
+@pytest.mark.parametrize("dtype,q_lens,ctx_lens,options", NAN_BATCHES)
+def test_accumulate_attention_over_a_key_that_is_nan(dtype, q_lens, ctx_lens, options, monkeypatch):
+    """Every key of the rows that see it becomes NaN: their softmax's sum is."""
+    Hq, Hkv, D = 4, 2, 128
+    c = _weights_case(dtype, Hq, Hkv, D, 16, q_lens, ctx_lens, 701)
+    window = options.get("window", 0)
+    monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_TC", options.get("tc", True))
+    clean = _gather(c, window, **{k: v for k, v in options.items() if k == "softcap"})[0]
+    total, ctx0 = q_lens[0] + ctx_lens[0], ctx_lens[0]
+    key = torch.arange(total)
+    for j in list(range(0, min(total, 19))) + [ctx0, total - 1]:
+        d = dict(c, pages=c["pages"].clone())
+        d["pages"][int(c["table"][0, j // 16]), 0, 1, j % 16, 9] = math.nan
+        seen = torch.zeros(total, dtype=torch.bool)
+        for i in range(q_lens[0]):
+            pos = ctx0 + i
+            if j <= pos and (not window or j > pos - window):
+                seen |= (key <= pos) & ((key > pos - window) if window else torch.ones(total, dtype=torch.bool))
+        _check_nan(d, clean, j, 2, seen, monkeypatch, options)
