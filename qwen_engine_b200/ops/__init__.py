@@ -1795,6 +1795,10 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
     for t in (slopes, sinks):
         _need(t is None or (t.dtype == torch.float32 and t.numel() == Hq and t.is_contiguous()), "accumulate_attention: slopes and sinks must be float32 [Hq]")
     _need(scale > 0.0 and softcap >= 0.0, "accumulate_attention: the scale must be positive, the cap not negative")
+    _need(len(ctx.q_lens_host) == R and len(ctx.ctx_lens_host) == R, "accumulate_attention: the context must have the lengths of every request")
+    for t, n in ((ctx.cu_q, R + 1), (ctx.ctx_lens, R), (ctx.slot_ids, R), (ctx.positions, T)):
+        _need(t.dtype == torch.int32 and t.numel() >= n and t.is_contiguous(),
+              "accumulate_attention: the context's cu_q [R + 1], ctx_lens [R], slot_ids [R] and positions [T] must be contiguous int32")
     page = int(kv_pages.shape[3])
     longest = max((q + c for q, c in zip(ctx.q_lens_host, ctx.ctx_lens_host)), default=0)
     if longest > weights.shape[2] or longest > block_tables.shape[1] * page:
