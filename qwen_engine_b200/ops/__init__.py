@@ -2636,9 +2636,9 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, draft_logits
     tokens int32 [N]: the request's rows get the drafts that stand, the drawn token, and -1 behind it; counts int32 [R]: how many
     tokens that are, a + 1 (so many of the request's rows are now part of its text).  A draft outside the vocabulary falls; NaN
     counts as -inf; a row without any logit above -inf lets no draft stand and gives token 0.  ``alloc(shape, dtype)`` gives scratch memory."""
+    _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.is_contiguous(), "verify_drafts: logits must be contiguous float32 [N, V]")
     N, V = logits.shape
     R = counts.numel()
-    _need(logits.dtype == torch.float32 and logits.is_contiguous(), "verify_drafts: logits must be contiguous float32 [N, V]")
     for t, n in ((draft_tokens, N - R), (row_starts, R + 1), (top_k, R), (tokens, N), (counts, R)):
         _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
               "verify_drafts: draft_tokens [N - R], row_starts [R + 1], top_k [R], tokens [N] and counts [R] must be contiguous int32")

@@ -149,3 +149,8 @@ def test_accumulate_attention_refuses_a_context_that_does_not_fit(name, value):
     setattr(args["ctx"], name, value)
     with pytest.raises(ops.KernelRefused, match="accumulate_attention"):
         ops.accumulate_attention(**args)
+
+
+def test_logits_that_are_no_rows_are_refused():
+    with pytest.raises(ops.KernelRefused):
+        ops.verify_drafts(**_verify_args(logits=torch.zeros(55)))
