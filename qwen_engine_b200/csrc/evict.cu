@@ -33,7 +33,7 @@ struct EvArgs {
   long head_stride;              // capacity: entries between a (layer, slot, head)'s row and the next
   int slots, Hkv, R, capacity, keep, first, recent;
   char* cache; int planes, page, row_bytes;
-  int* moves;                    // [layer, request, head]: 1 + 2 keep ints: how many, the places they come from, the places they go to
+  int* moves; int most;          // [layer, request, head]: 1 + 2 most ints: how many, the places they come from, the places they go to; most: min(keep, capacity - keep)
 };
 
 __device__ __forceinline__ unsigned ev_key(float w) {
@@ -63,7 +63,7 @@ __device__ __forceinline__ void ev_move(const EvArgs& A, int layer, int r, int h
     char *f = nullptr, *t = nullptr;
     if (lane < batch && i + lane < n) {
       f = place(__ldcg(moves + 1 + i + lane));
-      t = place(__ldcg(moves + 1 + A.keep + i + lane));
+      t = place(__ldcg(moves + 1 + A.most + i + lane));
       if (f == nullptr || t == nullptr) f = t = nullptr;
     }
     const int m = min(batch, n - i);
@@ -106,7 +106,7 @@ evict_select_kernel(EvArgs A, int held) {
   const int r = blockIdx.y / A.Hkv, h = blockIdx.y - r * A.Hkv, layer = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slot = A.slot_ids[r];
-  int* moves = A.moves + (((size_t)layer * A.R + r) * A.Hkv + h) * (size_t)(1 + 2 * A.keep);
+  int* moves = A.moves + (((size_t)layer * A.R + r) * A.Hkv + h) * (size_t)(1 + 2 * A.most);
   if (slot < 0 || slot >= A.slots) {            // no such slot: nothing is read or written (the whole cluster)
     if (rank == 0 && tid == 0) moves[0] = 0;
     return;
@@ -290,7 +290,7 @@ evict_select_kernel(EvArgs A, int held) {
     const unsigned head = j + 32 <= keep ? 0xffffffffu : (j >= keep ? 0u : (1u << (keep - j)) - 1u);
     const unsigned valid = j + 32 <= j1 ? 0xffffffffu : (1u << (j1 - j)) - 1u;
     const unsigned hb = ~sb & head & valid, mb = sb & ~head;
-    if ((hb >> lane) & 1u) moves[1 + keep + holes + __popc(hb & below)] = j + lane;
+    if ((hb >> lane) & 1u) moves[1 + A.most + holes + __popc(hb & below)] = j + lane;
     if ((mb >> lane) & 1u) moves[1 + movers + __popc(mb & below)] = j + lane;
     holes += __popc(hb);
     movers += __popc(mb);
@@ -302,7 +302,7 @@ evict_select_kernel(EvArgs A, int held) {
   __threadfence();
   cluster_sync_all();                           // both lists are whole, and nobody's shared memory is read any more
   for (int i = rank * EV_THREADS + tid; i < all_movers; i += C * EV_THREADS) {
-    const int from = __ldcg(moves + 1 + i), to = __ldcg(moves + 1 + keep + i);
+    const int from = __ldcg(moves + 1 + i), to = __ldcg(moves + 1 + A.most + i);
     Wo[to] = W[from];
     Po[to] = P[from];
   }
@@ -317,7 +317,7 @@ evict_move_kernel(EvArgs A, int batch) {
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.y / A.Hkv, h = blockIdx.y - r * A.Hkv, layer = blockIdx.z;
-  const int* moves = A.moves + (((size_t)layer * A.R + r) * A.Hkv + h) * (size_t)(1 + 2 * A.keep);
+  const int* moves = A.moves + (((size_t)layer * A.R + r) * A.Hkv + h) * (size_t)(1 + 2 * A.most);
   ev_move<V>(A, layer, r, h, moves, moves[0], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8, batch);
 }
 
@@ -346,8 +346,9 @@ extern "C" int qe_evict_tokens(void* cache, int layers, int num_pages, int plane
   if (layers <= 0 || R <= 0 || Hkv <= 0) return 0;
   if (keep < 1 || first < 0 || recent < 0) QE_REFUSE("evict_tokens: a budget of %d with %d first and %d recent entries", keep, first, recent);
   if ((long)R * Hkv > 65535 || layers > 65535) QE_REFUSE("evict_tokens: %d requests of %d heads, %d layers are more than a launch takes", R, Hkv, layers);
+  const int most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
   EvArgs args{block_tables, max_blocks, num_pages, slot_ids, lens, weights, positions, weights_out, positions_out, head_stride,
-              slots, Hkv, R, capacity, keep, first, recent, (char*)cache, planes, page_size, row_bytes, moves};
+              slots, Hkv, R, capacity, keep, first, recent, (char*)cache, planes, page_size, row_bytes, moves, most};
   // CTAs a head: one, where the heads of all layers and requests are as many as the SMs (a cluster's meetings cost more than a longer run of
   // entries: 128 heads of 32 768 entries, 8 CTAs each 90 us), else up to EV_MAX_CTAS; and as many as hold the keys
   unsigned ctas = 1;
@@ -358,7 +359,6 @@ extern "C" int qe_evict_tokens(void* cache, int layers, int num_pages, int plane
   const size_t smem = held ? per * 4 + per / 8 : 0;
   const dim3 select((unsigned)ctas, (unsigned)(R * Hkv), (unsigned)layers);
   // a few moves are made by the kernel that lists them: one launch less
-  const int most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
   const int unit = row_bytes % 16 == 0 && ((uintptr_t)cache & 15) == 0 ? 16 : (row_bytes % 4 == 0 && ((uintptr_t)cache & 3) == 0 ? 4 : 2);
   const bool inside = most <= EV_MOVES_INSIDE;
   cudaError_t e;

@@ -1891,7 +1891,7 @@ def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torc
         return
     capacity = min(weights.shape[3], block_tables.shape[1] * page)
     keep = min(int(keep), max(capacity, 1))
-    moves = alloc((S, R, Hkv, 1 + 2 * keep), torch.int32)
+    moves = alloc((S, R, Hkv, 1 + 2 * max(0, min(keep, capacity - keep))), torch.int32)       # (where from and where to)
     _check(_entry("qe_evict_tokens")(
         pc, S, pages, planes, Hkv, page, D * cache.element_size(), pt, block_tables.shape[1], psl, pl, R, pw, pp, pwo, ppo, weights.shape[1],
         weights.shape[3], capacity, keep, int(first), int(recent), moves.data_ptr(), _stream()), "evict_tokens")

@@ -818,3 +818,23 @@ def test_accumulate_attention_over_a_key_that_is_nan(dtype, q_lens, ctx_lens, op
             if j <= pos and (not window or j > pos - window):
                 seen |= (key <= pos) & ((key > pos - window) if window else torch.ones(total, dtype=torch.bool))
         _check_nan(d, clean, j, 2, seen, monkeypatch, options)
+
+
+# ---- scratch memory ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lens,keep", [([65, 60], 64), ([500, 130], 120), ([40], 400)])
+def test_evict_tokens_asks_for_scratch_memory_by_what_may_move(lens, keep):
+    """Two numbers for every entry that can move, min(keep, places - keep) a head at most, and one for how many do."""
+    c = _evict_case(torch.bfloat16, 2, 3, 16, 16, lens, 12)
+    d = {k: v.to(DEV) for k, v in c.items()}
+    asked = []
+
+    def alloc(shape, dtype):
+        asked.append(math.prod(shape))
+        return _alloc(shape, dtype)
+    wo, po = torch.zeros_like(d["weights"]), torch.zeros_like(d["positions"])
+    want = plain_drafts.evict(c["cache"], c["table"], c["slot_ids"], c["lens"], c["weights"], c["positions"], wo.cpu(), po.cpu(), keep, 2, 9)
+    ops.evict_tokens(d["cache"], d["table"], d["slot_ids"], d["lens"], d["weights"], d["positions"], wo, po, keep, 2, 9, alloc)
+    assert torch.equal(po.cpu(), want[2]) and torch.equal(wo.cpu(), want[1]) and torch.equal(d["cache"].cpu(), want[0])
+    places = min(c["weights"].shape[3], c["table"].shape[1] * 16)
+    assert sum(asked) <= 2 * len(lens) * 3 * (1 + 2 * max(0, min(keep, places - keep)))
