@@ -13,7 +13,9 @@
 //
 // Two forms.  Where a request's scores fit the shared memory of a cluster (parts of its keys, a CTA each), the CTAs keep them
 // there, exchange their rows' maxima and sums through distributed shared memory, and finish their keys: one launch, nothing
-// but keys and weights through memory.  Else the scores go to scratch memory and a second kernel adds them up.
+// but keys and weights through memory.  Else the scores go to scratch memory and a second kernel adds them up.  Scratch memory goes by the widths of slots
+// and tables (a captured call is replayed with other lengths) as long as that is little; beyond, the requests' scores lie one behind the other, and what
+// finds no room is formed twice (32 x 5 rows, 8 000 to 1 800 keys held in 131 072 places, 242 us with 0.27 GB of scratch memory for 205 with 2.7).
 //
 // What bounds them: the keys, from memory (4 requests of 131 071 keys, 32 / 8 heads of 128: 1.07 GB in 205 us, 5.2 TB/s, and 23 us for the second kernel);
 // with more rows a key the scores' way through L2 and their instructions (32 x 5 rows behind up to 8 200 keys 77 us); with few keys the launch
@@ -43,7 +45,7 @@ __device__ __forceinline__ uint4 af_ld_key(const void* p, uint64_t policy) {
 }
 
 // The scores of the CTA's keys [key0, key1) (key0 a multiple of 32) against the request's rows, in units of log2(e), -inf where
-// a row may not see a key: S[row * ld + key - key0]; and the rows' maxima and sums over those keys into row_max / row_sum (of all MT x 16 rows).
+// a row may not see a key: S[row * ld + key - key0] (null: nowhere); and the rows' maxima and sums over those keys into row_max / row_sum (of all MT x 16 rows).
 // MT: tiles of 16 rows; PLAIN: scores are neither bent nor biased.  A warp goes through its keys 64 channels at a time, the next 64 (of the same
 // 32 keys or of its next ones) on their way while these are multiplied.
 template <int MT, bool PLAIN>
@@ -182,7 +184,7 @@ __device__ __forceinline__ void af_scores(const AwArgs& A, const AwReq& R, int r
             if (!(((held >> e) & 1u) && key <= p && (A.window <= 0 || key > p - A.window))) v[e] = -INFINITY;
           }
         }
-        if (rho < rows) {
+        if (rho < rows && S != nullptr) {
           float4* dst = reinterpret_cast<float4*>(S + rho * ld + (j0 - key0) + 8 * x);
           dst[0] = make_float4(v[0], v[1], v[2], v[3]);
           dst[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -307,29 +309,68 @@ attention_weights_cluster_kernel(AwArgs A, int max_rows, int part_keys) {
 
 // ---- the scores through scratch memory -------------------------------------------------------------------------------------------
 
-// scores: [request, kv head, max_rows, ld]
+// Where a request's scores lie: element (head, row, key - af_first) at base + (head * rows + row) * ld + key - af_first, base < 0 where they are not kept.
+struct AfPlace { long base, ld; int rows; };
+
+// ld > 0: [request, kv head, max_rows, ld].  ld == 0: the requests' scores one behind the other, as many floats as each has, as far as `room` reaches: memory by
+// what is held and not by the widths of slots and tables; a request that finds no room is formed again by attention_weights_again_kernel.
+__device__ __forceinline__ AfPlace af_place(const AwArgs& A, const AwReq& R, int r, int max_rows, long ld, long room, long* sums) {
+  if (ld > 0) return AfPlace{(long)r * A.Hkv * max_rows * ld, ld, max_rows};
+  const int G = A.Hq / A.Hkv, tid = threadIdx.x;
+  auto width = [&](const AwReq& Q) { return (long)((Q.total - af_first(A, Q) + AF_GROUP - 1) / AF_GROUP * AF_GROUP); };
+  long before = 0;
+  for (int i = tid; i < r; i += AF_THREADS) {
+    const AwReq Q = aw_req(A, i);
+    if (af_mine(A, Q, max_rows)) before += width(Q) * (Q.counted * G);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if ((tid & 31) == 0) sums[tid >> 5] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < AF_WARPS; ++w) before += sums[w];
+  before *= A.Hkv;
+  const long own = width(R) * (R.counted * G);
+  return AfPlace{before + own * A.Hkv <= room ? before : -1, width(R), R.counted * G};
+}
+
+// stats: [request, kv head, max_rows, parts, 2]
+__device__ __forceinline__ float* af_stats(const AwArgs& A, int r, int c, int max_rows, int row) {
+  return A.stats + (((size_t)r * A.Hkv + c) * max_rows + row) * A.parts * 2;
+}
+
+// the keys of a part: at least least_keys, a multiple of 32, so that a short request has fewer parts
+__device__ __forceinline__ int2 af_part(const AwArgs& A, const AwReq& R, int part, int least_keys) {
+  const int first = af_first(A, R);
+  const int per = (max((R.total - first + A.parts - 1) / A.parts, least_keys) + AF_GROUP - 1) / AF_GROUP * AF_GROUP;
+  const int key0 = min(first + part * per, R.total);
+  return make_int2(key0, min(key0 + per, R.total));
+}
+
 template <int MT, bool PLAIN>
 __global__ void __launch_bounds__(AF_THREADS, 2)
-attention_weights_scores_kernel(AwArgs A, int max_rows, int least_keys, float* scores, long ld) {
+attention_weights_scores_kernel(AwArgs A, int max_rows, int least_keys, float* scores, long ld, long room) {
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ float warp_ml[AF_WARPS][MT * 16][2];
   __shared__ float row_max[MT * 16], row_sum[MT * 16];
+  __shared__ long sums[AF_WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const int part = blockIdx.x, c = blockIdx.y, r = blockIdx.z, tid = threadIdx.x;
   const AwReq R = aw_req(A, r);
   if (!af_mine(A, R, max_rows)) return;
   const int G = A.Hq / A.Hkv, rows = R.counted * G;
-  const int first = af_first(A, R);
-  const int per = (max((R.total - first + A.parts - 1) / A.parts, least_keys) + AF_GROUP - 1) / AF_GROUP * AF_GROUP;
-  const int key0 = min(first + part * per, R.total), key1 = min(key0 + per, R.total);
-  float* st = A.stats + ((size_t)(R.row0 + tid / G) * A.Hq + c * G + tid % G) * A.parts * 2 + part * 2;      // of row tid
-  if (key0 == key1) {                             // (a short request has fewer parts)
+  const int2 keys = af_part(A, R, part, least_keys);
+  const int key0 = keys.x, key1 = keys.y;
+  float* st = af_stats(A, r, c, max_rows, min(tid, max_rows - 1)) + part * 2;      // of row tid
+  if (key0 == key1) {
     if (tid < rows) { st[0] = -INFINITY; st[1] = 0.f; }
     return;
   }
-  float* S = scores + (((size_t)r * A.Hkv + c) * max_rows) * ld + (key0 - first);
-  af_scores<MT, PLAIN>(A, R, r, c, key0, key1, S, ld, reinterpret_cast<uint4*>(raw), warp_ml, row_max, row_sum);
+  const AfPlace place = af_place(A, R, r, max_rows, ld, room, sums);
+  float* S = place.base < 0 ? nullptr : scores + place.base + (long)c * place.rows * place.ld + (key0 - af_first(A, R));
+  af_scores<MT, PLAIN>(A, R, r, c, key0, key1, S, place.ld, reinterpret_cast<uint4*>(raw), warp_ml, row_max, row_sum);
   if (tid < rows) {
     st[0] = row_max[tid];
     st[1] = row_sum[tid];
@@ -337,8 +378,9 @@ attention_weights_scores_kernel(AwArgs A, int max_rows, int least_keys, float* s
 }
 
 __global__ void __launch_bounds__(AF_THREADS)
-attention_weights_sum_kernel(AwArgs A, int max_rows, const float* __restrict__ scores, long ld) {
+attention_weights_sum_kernel(AwArgs A, int max_rows, const float* __restrict__ scores, long ld, long room) {
   __shared__ float2 row[32];
+  __shared__ long sums[AF_WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const int c = blockIdx.y, r = blockIdx.z, tid = threadIdx.x;
@@ -346,19 +388,17 @@ attention_weights_sum_kernel(AwArgs A, int max_rows, const float* __restrict__ s
   const int slot = A.slot_ids[r];
   if (!af_mine(A, R, max_rows) || slot < 0 || slot >= A.slots || (int)blockIdx.x * AF_THREADS * 4 >= R.total) return;
   const int G = A.Hq / A.Hkv, rows = R.counted * G, first = af_first(A, R);
-  if (tid < rows) {
-    const int t = tid / G, head = c * G + (tid - t * G);
-    row[tid] = aw_merge(A.stats + ((size_t)(R.row0 + t) * A.Hq + head) * A.parts * 2, A.parts, A.sinks ? A.sinks + head : nullptr);
-  }
+  if (tid < rows) row[tid] = aw_merge(af_stats(A, r, c, max_rows, tid), A.parts, A.sinks ? A.sinks + c * G + tid % G : nullptr);
+  const AfPlace place = af_place(A, R, r, max_rows, ld, room, sums);
   __syncthreads();
   const int k0 = (blockIdx.x * AF_THREADS + tid) * 4;
-  if (k0 >= R.total) return;
-  const float* S = scores + (((size_t)r * A.Hkv + c) * max_rows) * ld + (k0 - first);
+  if (k0 >= R.total || (place.base < 0 && k0 >= first)) return;
+  const float* S = scores + place.base + (long)c * place.rows * place.ld + (k0 - first);
   float t[4] = {0.f, 0.f, 0.f, 0.f};
   if (k0 >= first) {                              // (first is a multiple of 32, rows of the scratch memory are whole runs of 32 keys)
 #pragma unroll 4
     for (int rho = 0; rho < rows; ++rho) {
-      const float4 s = __ldcs(reinterpret_cast<const float4*>(S + rho * ld));
+      const float4 s = __ldcs(reinterpret_cast<const float4*>(S + rho * place.ld));
       const float2 mz = row[rho];
       t[0] = fmaf(aw_ex2(s.x - mz.x), mz.y, t[0]); t[1] = fmaf(aw_ex2(s.y - mz.x), mz.y, t[1]);
       t[2] = fmaf(aw_ex2(s.z - mz.x), mz.y, t[2]); t[3] = fmaf(aw_ex2(s.w - mz.x), mz.y, t[3]);
@@ -374,6 +414,43 @@ attention_weights_sum_kernel(AwArgs A, int max_rows, const float* __restrict__ s
   }
 }
 
+// The keys of requests whose scores found no room: their scores once more, AF_AGAIN keys of a part at a time into shared memory, and the sums.
+#define AF_AGAIN 512
+template <int MT, bool PLAIN>
+__global__ void __launch_bounds__(AF_THREADS, 2)
+attention_weights_again_kernel(AwArgs A, int max_rows, int least_keys, long room) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ float warp_ml[AF_WARPS][MT * 16][2];
+  __shared__ float row_max[MT * 16], row_sum[MT * 16];
+  __shared__ float2 row[MT * 16];
+  __shared__ long sums[AF_WARPS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int c = blockIdx.y, r = blockIdx.z, tid = threadIdx.x;
+  const AwReq R = aw_req(A, r);
+  const int slot = A.slot_ids[r];
+  if (!af_mine(A, R, max_rows) || slot < 0 || slot >= A.slots) return;
+  const int2 keys = af_part(A, R, blockIdx.x, least_keys);
+  if (keys.x == keys.y || af_place(A, R, r, max_rows, 0, room, sums).base >= 0) return;      // (the whole CTA)
+  const int G = A.Hq / A.Hkv, rows = R.counted * G;
+  if (tid < rows) row[tid] = aw_merge(af_stats(A, r, c, max_rows, tid), A.parts, A.sinks ? A.sinks + c * G + tid % G : nullptr);
+  uint4* frags = reinterpret_cast<uint4*>(raw);
+  float* S = reinterpret_cast<float*>(frags + MT * ((A.D + 63) / 64 * 4) * 32);
+  const size_t base = ((size_t)slot * A.Hkv + c) * A.capacity;
+  for (int key0 = keys.x; key0 < keys.y; key0 += AF_AGAIN) {
+    const int key1 = min(key0 + AF_AGAIN, keys.y);
+    af_scores<MT, PLAIN>(A, R, r, c, key0, key1, S, AF_AGAIN + 4, frags, warp_ml, row_max, row_sum);
+    for (int key = key0 + tid; key < key1; key += AF_THREADS) {
+      float t = 0.f;
+#pragma unroll 4
+      for (int rho = 0; rho < rows; ++rho) t = fmaf(aw_ex2(S[rho * (AF_AGAIN + 4) + (key - key0)] - row[rho].x), row[rho].y, t);
+      A.out[base + key] = key < R.ctx ? A.weights[base + key] + t : t;
+      if (A.positions && key >= R.ctx) A.positions[base + key] = A.step_positions[R.row0 + key - R.ctx];
+    }
+    __syncthreads();                              // S and the queries' fragments are written anew
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 
 static size_t af_frag_bytes(int mt, int D) { return (size_t)mt * ((D + 63) / 64) * 4 * 512; }
@@ -386,7 +463,7 @@ extern "C" long qe_attention_weights_few_smem(int max_rows, int D, int part_keys
 }
 
 template <int MT, bool PLAIN>
-static cudaError_t af_launch(const AwArgs& A, int max_rows, int ctas, int part_keys, size_t smem, float* scores, long ld, int max_total, cudaStream_t stream) {
+static cudaError_t af_launch(const AwArgs& A, int max_rows, int ctas, int part_keys, size_t smem, float* scores, long ld, long room, int max_total, cudaStream_t stream) {
   if (ctas > 0) {
     if (smem > 48 * 1024) {
       static bool configured = false;
@@ -409,22 +486,35 @@ static cudaError_t af_launch(const AwArgs& A, int max_rows, int ctas, int part_k
     }
   }
   cudaError_t e = qe_launch(attention_weights_scores_kernel<MT, PLAIN>, dim3((unsigned)A.parts, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), frag, stream,
-                            A, max_rows, part_keys, scores, ld);
+                            A, max_rows, part_keys, scores, ld, room);
   if (e != cudaSuccess) return e;
-  return qe_launch(attention_weights_sum_kernel, dim3((unsigned)((max_total + AF_THREADS * 4 - 1) / (AF_THREADS * 4)), (unsigned)A.Hkv, (unsigned)A.R),
-                   dim3(AF_THREADS), 0, stream, A, max_rows, (const float*)scores, ld);
+  e = qe_launch(attention_weights_sum_kernel, dim3((unsigned)((max_total + AF_THREADS * 4 - 1) / (AF_THREADS * 4)), (unsigned)A.Hkv, (unsigned)A.R),
+                dim3(AF_THREADS), 0, stream, A, max_rows, (const float*)scores, ld, room);
+  if (e != cudaSuccess || ld > 0) return e;
+  const size_t again = frag + (size_t)max_rows * (AF_AGAIN + 4) * 4;
+  if (again > 48 * 1024) {
+    static bool configured = false;
+    if (!configured) {
+      e = cudaFuncSetAttribute(attention_weights_again_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 180 * 1024);
+      if (e != cudaSuccess) return e;
+      configured = true;
+    }
+  }
+  return qe_launch(attention_weights_again_kernel<MT, PLAIN>, dim3((unsigned)A.parts, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), again, stream,
+                   A, max_rows, part_keys, room);
 }
 
 // The requests of at most `max_rows` rows (a query token x a query head of a kv head's group), 32 at most.  ctas > 0: clusters of so many
 // CTAs (1, 2, 4, 8) hold the scores, part_keys keys a CTA at most (a multiple of 32; span <= ctas part_keys); 0: parts of at least part_keys, and `scores`, scratch
-// memory of [R, Hkv, max_rows, ld] floats with ld a multiple of 4 and at least span + 32, does.  span: the most keys that a request's rows
+// memory of `room` floats, does: [R, Hkv, max_rows, ld] with ld a multiple of 32 and at least span, or, with ld == 0, whatever there is (af_place).
+// stats: [R, Hkv, max_rows, parts, 2].  span: the most keys that a request's rows
 // see between them, from a multiple of 32 on (max_total without a window).
 extern "C" int qe_attention_weights_few(const void* q, long q_stride, int T, const void* pages, int num_pages, int planes,
                                         const int* block_tables, int max_blocks, const int* cu_q, const int* ctx_lens, const int* slot_ids,
                                         const int* counted, const int* step_positions, int* positions, const float* weights, float* out,
                                         int slots, long capacity, int R, int Hq, int Hkv, int D, int page, int window, float scale,
                                         float softcap, const float* slopes, const float* sinks, float* stats, int parts, int max_rows,
-                                        int max_total, int span, int ctas, int part_keys, float* scores, long ld, cudaStream_t stream) {
+                                        int max_total, int span, int ctas, int part_keys, float* scores, long ld, long room, cudaStream_t stream) {
   if (R <= 0 || max_total <= 0) return 0;
   if (Hkv < 1 || Hq % Hkv || page < 1) QE_REFUSE("attention_weights: heads %d/%d, pages of %d", Hq, Hkv, page);
   if (R > 65535 || Hkv > 65535) QE_REFUSE("attention_weights: %d requests, %d kv heads are more than a launch takes", R, Hkv);
@@ -432,14 +522,14 @@ extern "C" int qe_attention_weights_few(const void* q, long q_stride, int T, con
   if (smem == 0 || ((uintptr_t)pages & 15)) QE_REFUSE("attention_weights: %d rows of %d channels are not for the kernel of few rows", max_rows, D);
   if (ctas > 0 && (ctas > AF_MAX_CTAS || (ctas & (ctas - 1)) || part_keys % AF_GROUP || (long)ctas * part_keys < span || smem > 220 * 1024))
     QE_REFUSE("attention_weights: %d CTAs of %d keys for %d", ctas, part_keys, span);
-  if (ctas == 0 && (scores == nullptr || stats == nullptr || parts < 1 || ld % 4 || ld < span + AF_GROUP))
+  if (ctas == 0 && (scores == nullptr || stats == nullptr || parts < 1 || ld % AF_GROUP || (ld != 0 && (ld < span || room / ld / max_rows / Hkv < R))))
     QE_REFUSE("attention_weights: scratch memory for %d keys is needed", span);
   AwArgs A{q, q_stride, T, pages, num_pages, planes, block_tables, max_blocks, cu_q, ctx_lens, slot_ids, counted, step_positions, positions,
            weights, out, slots, capacity, R, Hq, Hkv, D, page, aw_shift(page), window, scale, softcap, slopes, sinks, stats, parts};
   const bool plain = softcap <= 0.f && slopes == nullptr;
   cudaError_t e;
-  if (max_rows > 16) e = plain ? af_launch<2, true>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream) : af_launch<2, false>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream);
-  else e = plain ? af_launch<1, true>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream) : af_launch<1, false>(A, max_rows, ctas, part_keys, smem, scores, ld, max_total, stream);
+  if (max_rows > 16) e = plain ? af_launch<2, true>(A, max_rows, ctas, part_keys, smem, scores, ld, room, max_total, stream) : af_launch<2, false>(A, max_rows, ctas, part_keys, smem, scores, ld, room, max_total, stream);
+  else e = plain ? af_launch<1, true>(A, max_rows, ctas, part_keys, smem, scores, ld, room, max_total, stream) : af_launch<1, false>(A, max_rows, ctas, part_keys, smem, scores, ld, room, max_total, stream);
   if (e != cudaSuccess) { qe_set_error("attention_weights: launch failed: %s", cudaGetErrorString(e)); (void)cudaGetLastError(); return 2; }
   QE_CHECK_LAUNCH("attention_weights");
   return 0;

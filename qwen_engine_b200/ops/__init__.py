@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 import math
+import operator
 import os
 import struct
 import weakref
@@ -1696,7 +1697,7 @@ _P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long
 _AW_ARGS = [_P, _L, _I, _P, _I, _I, _P, _I] + [_P] * 8 + [_I, _L] + [_I] * 6 + [_F, _F, _P, _P]
 _SIGNATURES = {       # entry points that are called with plain numbers (ctypes converts them by these types)
     "qe_attention_weights": _AW_ARGS + [_P] + [_I] * 5 + [_P, _I, _P],
-    "qe_attention_weights_few": _AW_ARGS + [_P] + [_I] * 6 + [_P, _L, _P],
+    "qe_attention_weights_few": _AW_ARGS + [_P] + [_I] * 6 + [_P, _L, _L, _P],
     "qe_attention_weights_tc": _AW_ARGS + [_P, _I, _I, _P, _P, _I, _I, _I, _P],
     "qe_evict_tokens": [_P] + [_I] * 6 + [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _L] + [_I] * 4 + [_P, _P],
     "qe_verify_drafts": [_P] * 11 + [_I] * 3 + [_P],
@@ -1741,6 +1742,11 @@ def attention_weights_cluster(rows: int, heads: int, head_dim: int, requests: in
     return 0, min(2048, max(512, -(-requests * heads * span // (256 * 32)) * 32))
 
 
+ATTENTION_WEIGHTS_SCRATCH = 1 << 28           # bytes of scratch memory for a few rows' scores, or for the parts of the keys' sums: where they would be more by the
+                                              # widths of slots and tables (64 requests of 32 rows in tables of 131 072 places: 8.6 GB), the scores take what the
+ATTENTION_WEIGHTS_SCRATCH_MOST = 1 << 30      # held lengths need, this at most; what finds no room is formed twice
+
+
 ATTENTION_WEIGHTS_TC = True                   # more rows in bfloat16: the kernels on the tensor cores (False: the general kernels serve them)
 
 
@@ -1748,6 +1754,20 @@ def attention_weights_tc_parts(units: int, tiles: int) -> int:
     """In how many parts each unit's walk over ``tiles`` tiles is cut: a unit an SM (with four: a prompt of 4 096 tokens, 32 / 8 heads,
     239 us for 217, 64 tokens behind 32 000 112 for 95), four tiles a part at least."""
     return max(1, min(-(-TC_TARGET_CTAS // max(1, units)), -(-tiles // 4), ATTENTION_WEIGHTS_MAX_PARTS))
+
+
+def _some_requests(args: tuple, blocks: int, wanted: list) -> tuple[tuple, int]:
+    """The arguments (_AW_ARGS) of the requests from the first to the last of those that are wanted, and how many they are: launches and scratch memory for
+    those alone (one prompt of 1 000 tokens among 47 requests of one, 16 384 places: 99 us for 897).  2 us of the host's time, so not for a handful of requests."""
+    r0 = wanted.index(True)
+    nr = len(wanted) - r0 - wanted[::-1].index(True)
+    a = list(args)
+    a[6] += 4 * r0 * blocks                       # block tables
+    for i in (8, 9, 10, 11):                      # first rows, cached tokens, slots, rows that count
+        if a[i] is not None:
+            a[i] += 4 * r0
+    a[18] = nr
+    return tuple(a), nr
 
 
 def _cluster_smem(rows: int, head_dim: int, part: int) -> int:
@@ -1771,85 +1791,99 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
     the others' keys get no weight.
     ``window``, ``slopes``, ``softcap``, ``sinks``: as in ``paged_attention``.  Keys that lie in no page get no weight; distances
     are of places in the cache, so that a window or a distance bias goes with a cache that nothing was evicted from.
-    ``alloc(shape, dtype)`` gives scratch memory.  Float32 sums in one order: equal calls give equal bits.  Launches go by the
+    ``alloc(shape, dtype)`` gives scratch memory, ATTENTION_WEIGHTS_SCRATCH bytes of it for scores or sums (more, up to ATTENTION_WEIGHTS_SCRATCH_MOST, where the
+    lengths that ctx.ctx_lens_host holds need it).  Float32 sums in one order: equal calls give equal bits.  Launches go by the
     requests' tokens (ctx.q_lens_host): a captured call may be replayed with other cached lengths, pages, slots and ``counted``
     on the device, not with other numbers of tokens."""
     Hq, Hkv, D = num_heads, num_kv_heads, head_dim
-    T, R, planes = qkv.shape[0], int(ctx.num_reqs), int(kv_pages.shape[1]) if kv_pages.dim() == 5 else 0
     _rows(qkv, "accumulate_attention: qkv")
+    (T, columns), R, kv_shape, shape = qkv.shape, int(ctx.num_reqs), kv_pages.shape, weights.shape
     _need(Hkv >= 1 and Hq % Hkv == 0 and D >= 1, "accumulate_attention: the query heads must be a multiple of the kv heads")
-    _need(qkv.shape[1] >= Hq * D, "accumulate_attention: qkv must hold Hq D columns of queries")
-    _need(kv_pages.dtype == qkv.dtype and kv_pages.dim() == 5 and kv_pages.is_contiguous() and planes >= 1
-          and kv_pages.shape[2] == Hkv and kv_pages.shape[4] == D,
+    _need(columns >= Hq * D, "accumulate_attention: qkv must hold Hq D columns of queries")
+    _need(kv_pages.dtype == qkv.dtype and len(kv_shape) == 5 and kv_pages.is_contiguous() and kv_shape[1] >= 1 and kv_shape[2] == Hkv and kv_shape[4] == D,
           "accumulate_attention: kv_pages must be [pages, planes, Hkv, page, D] in q's dtype")
     _i32(block_tables, "block_tables")
     _need(block_tables.dim() == 2 and block_tables.shape[0] == R, "accumulate_attention: block_tables must be [R, blocks]")
-    _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[1] == Hkv and weights.is_contiguous()
-          and out.dtype == torch.float32 and out.shape == weights.shape and out.is_contiguous(),
+    _need(weights.dtype == torch.float32 and len(shape) == 3 and shape[1] == Hkv and weights.is_contiguous()
+          and out.dtype == torch.float32 and out.shape == shape and out.is_contiguous(),
           "accumulate_attention: weights and out must be contiguous float32 [slots, Hkv, capacity]")
-    _need(_same_or_apart(weights, out), "accumulate_attention: weights and out must be one tensor or share no memory")
-    _need(positions is None or (positions.dtype == torch.int32 and positions.shape == weights.shape and positions.is_contiguous()),
+    _need(out is weights or _same_or_apart(weights, out), "accumulate_attention: weights and out must be one tensor or share no memory")
+    _need(positions is None or (positions.dtype == torch.int32 and positions.shape == shape and positions.is_contiguous()),
           "accumulate_attention: positions must be int32 [slots, Hkv, capacity]")
     _need(counted is None or (counted.dtype == torch.int32 and counted.shape == (R,) and counted.is_contiguous()),
           "accumulate_attention: counted must be int32 [R]")
     for t in (slopes, sinks):
         _need(t is None or (t.dtype == torch.float32 and t.numel() == Hq and t.is_contiguous()), "accumulate_attention: slopes and sinks must be float32 [Hq]")
     _need(scale > 0.0 and softcap >= 0.0, "accumulate_attention: the scale must be positive, the cap not negative")
-    _need(len(ctx.q_lens_host) == R and len(ctx.ctx_lens_host) == R, "accumulate_attention: the context must have the lengths of every request")
+    q_lens, ctx_lens = ctx.q_lens_host, ctx.ctx_lens_host
+    _need(len(q_lens) == R and len(ctx_lens) == R, "accumulate_attention: the context must have the lengths of every request")
     for t, n in ((ctx.cu_q, R + 1), (ctx.ctx_lens, R), (ctx.slot_ids, R), (ctx.positions, T)):
-        _need(t.dtype == torch.int32 and t.numel() >= n and t.is_contiguous(),
-              "accumulate_attention: the context's cu_q [R + 1], ctx_lens [R], slot_ids [R] and positions [T] must be contiguous int32")
-    page = int(kv_pages.shape[3])
-    longest = max((q + c for q, c in zip(ctx.q_lens_host, ctx.ctx_lens_host)), default=0)
-    if longest > weights.shape[2] or longest > block_tables.shape[1] * page:
-        raise KernelRefused(f"accumulate_attention: a request of {longest} tokens in {int(block_tables.shape[1])} blocks of {page} and {int(weights.shape[2])} places")
+        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+            raise KernelRefused("accumulate_attention: the context's cu_q [R + 1], ctx_lens [R], slot_ids [R] and positions [T] must be contiguous int32")
+    pages, planes, _, page, _ = kv_shape
+    slots, _, capacity = shape
+    blocks = block_tables.shape[1]
+    longest = max(map(operator.add, q_lens, ctx_lens), default=0)
+    if longest > capacity or longest > blocks * page:
+        raise KernelRefused(f"accumulate_attention: a request of {longest} tokens in {blocks} blocks of {page} and {capacity} places")
     pq, pk, pt, pw, po, pn, pc, psl, psi, pcu, pctx, pslot, pstep = _operands(
         "accumulate_attention", qkv, kv_pages, block_tables, weights, out, positions, counted, slopes, sinks, ctx.cu_q, ctx.ctx_lens, ctx.slot_ids,
         ctx.positions)
     if R == 0:
         return
-    blocks, capacity = block_tables.shape[1], weights.shape[2]
-    max_total, G, max_q = min(capacity, blocks * page), Hq // Hkv, max(ctx.q_lens_host)
+    max_total, G, max_q = min(capacity, blocks * page), Hq // Hkv, max(q_lens)
     stream = _stream()
-    args = (pq, qkv.stride(0), T, pk, kv_pages.shape[0], planes, pt, blocks, pcu, pctx, pslot, pc, pstep, pn, pw, po, weights.shape[0], capacity, R,
+    args = (pq, qkv.stride(0), T, pk, pages, planes, pt, blocks, pcu, pctx, pslot, pc, pstep, pn, pw, po, slots, capacity, R,
             Hq, Hkv, D, page, int(window), scale, softcap, psl, psi)
     # the requests of a few rows, and the others
     few = -1
     if qkv.dtype == torch.bfloat16 and D % 8 == 0 and D <= 1024 and pk % 16 == 0:
-        few = max((max(n, 1) * G for n in ctx.q_lens_host if n * G <= ATTENTION_WEIGHTS_FEW_ROWS), default=-1)
+        few = max((max(n, 1) * G for n in q_lens if n * G <= ATTENTION_WEIGHTS_FEW_ROWS), default=-1)
         if few > ATTENTION_WEIGHTS_FEW_ROWS:     # (requests without a token, of more heads than that)
             few = ATTENTION_WEIGHTS_FEW_ROWS
     if few > 0:
         span = min(max_total, int(window) + few // G + 31) if window > 0 else max_total
-        ctas, part_keys = attention_weights_cluster(few, Hkv, D, R, span)
-        scores, ld, parts, stats = None, 0, 1, None
+        mine, nr = (args, R) if few >= max_q * G or R < 8 else _some_requests(args, blocks, [n * G <= few for n in q_lens])
+        ctas, part_keys = attention_weights_cluster(few, Hkv, D, nr, span)
+        scores, ld, room, parts, stats = None, 0, 0, 1, None
         if ctas == 0:
             parts = min(-(-span // part_keys), ATTENTION_WEIGHTS_MAX_PARTS)
-            ld = -(-(span + 32) // 32) * 32
-            scores, stats = alloc((R, Hkv, few, ld), torch.float32), alloc((max(T, 1) * Hq, parts, 2), torch.float32)
+            ld = -(-span // 32) * 32
+            room = nr * Hkv * few * ld
+            if 4 * room > ATTENTION_WEIGHTS_SCRATCH:
+                need = Hkv * sum(n * G * -(-min(n + c, span) // 32) * 32 for n, c in zip(q_lens, ctx_lens) if n * G <= few)
+                if 4 * room > min(8 * need, ATTENTION_WEIGHTS_SCRATCH_MOST):      # (a place for each is faster than one behind the other)
+                    ld, room = 0, max(32, min(max(4 * need, ATTENTION_WEIGHTS_SCRATCH), ATTENTION_WEIGHTS_SCRATCH_MOST) // 4)
+            scores, stats = alloc((room,), torch.float32), alloc((nr, Hkv, few, parts, 2), torch.float32)
         _check(_entry("qe_attention_weights_few")(
-            *args, None if stats is None else stats.data_ptr(), parts, few, max_total, span, ctas, part_keys,
-            None if scores is None else scores.data_ptr(), ld, stream), "accumulate_attention")
+            *mine, None if stats is None else stats.data_ptr(), parts, few, max_total, span, ctas, part_keys,
+            None if scores is None else scores.data_ptr(), ld, room, stream), "accumulate_attention")
         if few >= max_q * G:
             return
+    mine, nr = (args, R) if few < 0 or R < 8 else _some_requests(args, blocks, [n * G > few for n in q_lens])
+    most_parts = ATTENTION_WEIGHTS_SCRATCH // (4 * nr * Hkv * max_total + 4) or 1
     if (ATTENTION_WEIGHTS_TC and qkv.dtype == torch.bfloat16 and pq % 16 == 0 and qkv.stride(0) % 8 == 0 and qkv.stride(0) > 0 and pk % 16 == 0 and max_q > 0
             and lib().qe_attention_weights_tc_supported(Hq, Hkv, D, page)):
         tpt, na = 128 // G, 4 if D <= 128 else (2 if D <= 192 else 1)      # tokens of a tile of queries, tiles a unit
-        many = [(n, n + c) for n, c in zip(ctx.q_lens_host, ctx.ctx_lens_host) if n * G > few]
-        parts1 = attention_weights_tc_parts(sum(-(-n // (tpt * na)) for n, _ in many) * Hkv, -(-max_total // 128))
-        parts2 = attention_weights_tc_parts(sum(-(-t // (128 * na)) for _, t in many) * Hkv, -(-max_q // tpt))
-        stats, merged = alloc((T * Hq, parts1, 2), torch.float32), alloc((Hkv, T // tpt + R, 128), torch.float32)
-        sums = alloc((parts2, R, Hkv, max_total), torch.float32) if parts2 > 1 else None
+        units1 = units2 = 0
+        for n, c in zip(q_lens, ctx_lens):
+            if n * G > few:
+                units1 -= -n // (tpt * na)
+                units2 -= -(n + c) // (128 * na)
+        parts1 = attention_weights_tc_parts(units1 * Hkv, -(-max_total // 128))
+        parts2 = min(attention_weights_tc_parts(units2 * Hkv, -(-max_q // tpt)), most_parts)
+        stats, merged = alloc((T * Hq, parts1, 2), torch.float32), alloc((Hkv, T // tpt + nr, 128), torch.float32)
+        sums = alloc((parts2, nr, Hkv, max_total), torch.float32) if parts2 > 1 else None
         _check(_entry("qe_attention_weights_tc")(
-            *args, stats.data_ptr(), parts1, parts2, merged.data_ptr(), None if sums is None else sums.data_ptr(), max_q, max_total, few, stream),
+            *mine, stats.data_ptr(), parts1, parts2, merged.data_ptr(), None if sums is None else sums.data_ptr(), max_q, max_total, few, stream),
             "accumulate_attention")
     else:
         rows, keys = -(-max_q * G // 64), -(-max_total // 64)          # tiles of either, about
-        parts, parts2 = _attention_weights_parts(rows * Hkv * R, keys), _attention_weights_parts(keys * Hkv * R, rows)
+        parts, parts2 = _attention_weights_parts(rows * Hkv * nr, keys), min(_attention_weights_parts(keys * Hkv * nr, rows), most_parts)
         stats = alloc((max(T, 1) * Hq, parts, 2), torch.float32)
-        sums = alloc((parts2, R, Hkv, max_total), torch.float32) if parts2 > 1 else None
+        sums = alloc((parts2, nr, Hkv, max_total), torch.float32) if parts2 > 1 else None
         _check(_entry("qe_attention_weights")(
-            *args, stats.data_ptr(), parts, max_q, max_total, few, parts2, None if sums is None else sums.data_ptr(), _dt(qkv), stream), "accumulate_attention")
+            *mine, stats.data_ptr(), parts, max_q, max_total, few, parts2, None if sums is None else sums.data_ptr(), _dt(qkv), stream), "accumulate_attention")
 
 
 def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,

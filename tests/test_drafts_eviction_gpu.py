@@ -838,3 +838,72 @@ def test_evict_tokens_asks_for_scratch_memory_by_what_may_move(lens, keep):
     assert torch.equal(po.cpu(), want[2]) and torch.equal(wo.cpu(), want[1]) and torch.equal(d["cache"].cpu(), want[0])
     places = min(c["weights"].shape[3], c["table"].shape[1] * 16)
     assert sum(asked) <= 2 * len(lens) * 3 * (1 + 2 * max(0, min(keep, places - keep)))
+
+
+def _record(monkeypatch):
+    """The bytes that the calls from here on ask for as scratch memory, one number a piece."""
+    asked, plain = [], _alloc
+
+    def alloc(shape, dtype):
+        asked.append(math.prod(shape) * dtype.itemsize)
+        return plain(shape, dtype)
+    monkeypatch.setitem(globals(), "_alloc", alloc)
+    return asked
+
+
+def _widen(c, places, P):
+    """The same case in slots and block tables of so many places."""
+    table = torch.full((c["table"].shape[0], places // P), -1, dtype=torch.int32)
+    table[:, :c["table"].shape[1]] = c["table"]
+    return dict(c, table=table, weights=torch.nn.functional.pad(c["weights"], (0, places - c["weights"].shape[2])))
+
+
+def test_accumulate_attention_in_wide_tables_asks_for_bounded_scratch_memory(monkeypatch):
+    """One long request among many short ones in tables of 131 072 places: the scores of all would be 805 MB."""
+    q_lens = [4] * 23 + [3]
+    c = _widen(_weights_case(torch.bfloat16, 16, 2, 64, 16, q_lens, [3 + 11 * r for r in range(23)] + [9000], 800), 131072, 16)
+    asked = _record(monkeypatch)
+    _check_weights(c)
+    assert asked and max(asked) <= ops.ATTENTION_WEIGHTS_SCRATCH and sum(asked) <= 1.1 * ops.ATTENTION_WEIGHTS_SCRATCH
+    # ... and where more is held than that: what is held, up to a limit
+    c["q_lens"] = [4] * 24
+    c["ctx_lens"] = [131000] * 24
+    meta = lambda shape, dtype: asked.append(math.prod(shape) * dtype.itemsize) or torch.empty(4, dtype=dtype, device=DEV)
+    del asked[:]
+    monkeypatch.setattr(ops, "_entry", lambda name: lambda *a: 0)          # (asked for, not launched)
+    monkeypatch.setitem(globals(), "_alloc", meta)
+    c["cu"], c["qkv"] = torch.arange(0, 97, 4, dtype=torch.int32), torch.zeros(96, c["qkv"].shape[1], dtype=torch.bfloat16)
+    c["step_positions"] = torch.zeros(96, dtype=torch.int32)
+    _gather(c)
+    assert 0.9 * 4 * 24 * 2 * 32 * 131000 <= sum(asked) <= 1.1 * ops.ATTENTION_WEIGHTS_SCRATCH_MOST
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens", [([4, 1, 3, 4, 2], [600, 9, 5000, 40, 77]), ([4, 150, 0, 2, 90, 1], [600, 9, 50, 4000, 5, 0])])
+@pytest.mark.parametrize("Hq,D", [(12, 64), (24, 200)])
+@pytest.mark.parametrize("option", ["", "window", "sinks", "slopes"])
+def test_accumulate_attention_where_some_requests_scores_find_no_room(q_lens, ctx_lens, Hq, D, option, monkeypatch):
+    """Scratch memory for the scores of none, of some and of all requests: those that find no room are formed twice, with the same bits.  (Portions of more rows are cut into fewer parts
+    where their sums do not fit, and added up in another order: those are held against the definition alone.)"""
+    c = _weights_case(torch.bfloat16, Hq, 3, D, 16, q_lens, ctx_lens, 801, counted=[max(0, n - 1) for n in q_lens])
+    kw = {"window": dict(window=70), "sinks": dict(sinks=torch.randn(Hq)), "slopes": dict(slopes=torch.rand(Hq) * 0.1)}.get(option, {})
+    want = _check_weights(c, **kw)
+    longest = max(a + b for a, b in zip(q_lens, ctx_lens)) + 64
+    for heads in (0, 2, 3, 7, 10):
+        for name in ("ATTENTION_WEIGHTS_SCRATCH", "ATTENTION_WEIGHTS_SCRATCH_MOST"):
+            monkeypatch.setattr(ops, name, max(1, heads * 4 * 16 * longest))
+        got = _check_weights(c, **kw)
+        for n, slot in zip(q_lens, c["slots"].tolist()):
+            assert n * (Hq // 3) > ops.ATTENTION_WEIGHTS_FEW_ROWS or torch.equal(got[slot], want[slot])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_accumulate_attention_of_prompts_in_wide_tables_asks_for_bounded_scratch_memory(dtype, monkeypatch):
+    """A portion among requests of a few rows: parts of the keys' sums for the portion's own range of requests, and no parts where they would not fit."""
+    c = _widen(_weights_case(dtype, 8, 2, 64, 16, [1, 300, 1, 60] + [1] * 8, [50, 40, 700, 20] + [30] * 8, 802), 65536, 16)
+    asked = _record(monkeypatch)
+    _check_weights(c)
+    assert sum(asked) <= 2 * ops.ATTENTION_WEIGHTS_SCRATCH
+    del asked[:]
+    monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_SCRATCH", 1 << 16)
+    _check_weights(c)
+    assert sum(asked) <= 6 << 20                  # (the rows' statistics)
