@@ -466,24 +466,22 @@ template <int MT, bool PLAIN>
 static cudaError_t af_launch(const AwArgs& A, int max_rows, int ctas, int part_keys, size_t smem, float* scores, long ld, long room, int max_total, cudaStream_t stream) {
   if (ctas > 0) {
     if (smem > 48 * 1024) {
-      static bool configured = false;
-      if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attention_weights_cluster_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-        if (e != cudaSuccess) return e;
-        configured = true;
-      }
+      static unsigned long long configured = 0;
+      const cudaError_t e = qe_once_a_device(configured, [] {
+        return cudaFuncSetAttribute(attention_weights_cluster_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+      });
+      if (e != cudaSuccess) return e;
     }
     return qe_launch_cluster(attention_weights_cluster_kernel<MT, PLAIN>, dim3((unsigned)ctas, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), smem, stream,
                              (unsigned)ctas, A, max_rows, part_keys);
   }
   const size_t frag = af_frag_bytes(MT, A.D);
   if (frag > 48 * 1024) {
-    static bool configured = false;
-    if (!configured) {
-      cudaError_t e = cudaFuncSetAttribute(attention_weights_scores_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-      if (e != cudaSuccess) return e;
-      configured = true;
-    }
+    static unsigned long long configured = 0;
+    const cudaError_t e = qe_once_a_device(configured, [] {
+      return cudaFuncSetAttribute(attention_weights_scores_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    });
+    if (e != cudaSuccess) return e;
   }
   cudaError_t e = qe_launch(attention_weights_scores_kernel<MT, PLAIN>, dim3((unsigned)A.parts, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), frag, stream,
                             A, max_rows, part_keys, scores, ld, room);
@@ -493,12 +491,11 @@ static cudaError_t af_launch(const AwArgs& A, int max_rows, int ctas, int part_k
   if (e != cudaSuccess || ld > 0) return e;
   const size_t again = frag + (size_t)max_rows * (AF_AGAIN + 4) * 4;
   if (again > 48 * 1024) {
-    static bool configured = false;
-    if (!configured) {
-      e = cudaFuncSetAttribute(attention_weights_again_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 180 * 1024);
-      if (e != cudaSuccess) return e;
-      configured = true;
-    }
+    static unsigned long long configured = 0;
+    e = qe_once_a_device(configured, [] {
+      return cudaFuncSetAttribute(attention_weights_again_kernel<MT, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 180 * 1024);
+    });
+    if (e != cudaSuccess) return e;
   }
   return qe_launch(attention_weights_again_kernel<MT, PLAIN>, dim3((unsigned)A.parts, (unsigned)A.Hkv, (unsigned)A.R), dim3(AF_THREADS), again, stream,
                    A, max_rows, part_keys, room);

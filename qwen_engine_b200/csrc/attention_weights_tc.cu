@@ -471,12 +471,11 @@ template <int PASS, bool GENERAL>
 static cudaError_t at2_launch(dim3 grid, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const AwArgs& A, const AwTc& C) {
   const size_t smem = sizeof(AwTcSmem) + 1024;
   static_assert(tc_room_for_all(sizeof(AwTcSmem) + 1024, AT2_COLS), "tensor memory for every CTA that finds room on an SM");
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attention_weights_tc_kernel<PASS, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static unsigned long long configured = 0;
+  const cudaError_t e = qe_once_a_device(configured, [&] {
+    return cudaFuncSetAttribute(attention_weights_tc_kernel<PASS, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  });
+  if (e != cudaSuccess) return e;
   return qe_launch(attention_weights_tc_kernel<PASS, GENERAL>, grid, dim3(AT2_THREADS), smem, stream, q, k, A, C);
 }
 

@@ -96,6 +96,18 @@ __device__ __forceinline__ float glu_fast(float g, float u, int act) {
   return gate_act_fast(g, act) * u;
 }
 
+// Sets a kernel's attributes before its first launch on each device (they hold for one device; not at every launch: some are captured).
+// done: a bit for each device that has them.
+template <typename F>
+static inline cudaError_t qe_once_a_device(unsigned long long& done, F set) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || (device < 64 && ((done >> device) & 1ull))) return e;
+  e = set();
+  if (e == cudaSuccess && device < 64) done |= 1ull << device;
+  return e;
+}
+
 // ---- programmatic dependent launch --------------------------------------------------------------------
 // Kernels of a step form a chain on one stream.  Launched with the attribute below, a kernel may
 // start while its predecessor is still running; it must call pdl_wait() before it touches anything

@@ -323,11 +323,12 @@ evict_move_kernel(EvArgs A, int batch) {
 
 template <int MOVES, int THREADS>
 static cudaError_t ev_select_with(dim3 grid, size_t smem, cudaStream_t stream, const EvArgs& args, int held) {
-  static bool configured = false;
-  if (smem > 48 * 1024 && !configured) {
-    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<MOVES, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_SMEM);
+  if (smem > 48 * 1024) {
+    static unsigned long long configured = 0;
+    const cudaError_t e = qe_once_a_device(configured, [] {
+      return cudaFuncSetAttribute(evict_select_kernel<MOVES, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MAX_SMEM);
+    });
     if (e != cudaSuccess) return e;
-    configured = true;
   }
   return qe_launch_cluster(evict_select_kernel<MOVES, THREADS>, grid, dim3(THREADS), smem, stream, grid.x, args, held);
 }

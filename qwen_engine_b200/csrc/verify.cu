@@ -676,12 +676,9 @@ extern "C" int qe_verify_drafts(const float* logits, const int* draft_tokens, co
   while (ctas < VF_MAX_CTAS && rows * ctas < 1332 && V / (2 * ctas) >= 2048) ctas *= 2;
   while (draw < VF_MAX_DRAW && (long)R * draw < 148 && V / (2 * draw) >= 2048) draw *= 2;
   if (draw > 8) {
-    static bool configured = false;
-    if (!configured) {
-      cudaError_t e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) QE_REFUSE("verify_drafts: clusters of %u CTAs: %s", draw, cudaGetErrorString(e));
-      configured = true;
-    }
+    static unsigned long long configured = 0;
+    const cudaError_t e = qe_once_a_device(configured, [] { return cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
+    if (e != cudaSuccess) QE_REFUSE("verify_drafts: clusters of %u CTAs: %s", draw, cudaGetErrorString(e));
   }
   qe_launch_cluster(verify_sums_kernel, dim3((unsigned)(rows * ctas)), dim3(VF_THREADS), 0, stream, ctas, logits, draft_logits,
                     starts, temperature, top_k, (VfPart*)parts, thresholds, N, R, V);

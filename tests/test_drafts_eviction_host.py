@@ -154,3 +154,15 @@ def test_accumulate_attention_refuses_a_context_that_does_not_fit(name, value):
 def test_logits_that_are_no_rows_are_refused():
     with pytest.raises(ops.KernelRefused):
         ops.verify_drafts(**_verify_args(logits=torch.zeros(55)))
+
+
+def test_kernels_are_configured_for_every_device_they_run_on():
+    """A kernel's attributes hold for one device: no launcher of these operators sets them once a process."""
+    import os
+    import re
+    folder = os.path.join(os.path.dirname(os.path.abspath(ops.__file__)), "..", "csrc")
+    for name in ("verify.cu", "evict.cu", "attention_weights.cu", "attention_weights_few.cu", "attention_weights_tc.cu"):
+        source = open(os.path.join(folder, name)).read()
+        assert "static bool" not in source, name
+        for at in re.finditer("cudaFuncSetAttribute", source):
+            assert "qe_once_a_device(" in source[max(0, at.start() - 120):at.start()], name
