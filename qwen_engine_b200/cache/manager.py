@@ -61,6 +61,7 @@ class RequestCache:
     fresh_state: bool = True                              # its state rows must be zeroed before its first step
     closed: bool = False
     first_unknown: Optional[int] = None                   # position of a committed token whose id is not known yet
+    private: set[int] = field(default_factory=set)        # groups whose pages nobody else may hold or find (make_private)
 
 
 class CacheManager:
@@ -301,6 +302,8 @@ class CacheManager:
         P = self.page_size
         known = rc.num_tokens if rc.first_unknown is None else min(rc.num_tokens, rc.first_unknown)
         for g in self.paged_groups:
+            if g.index in rc.private:
+                continue
             table, chain = rc.tables[g.index], rc.hashes[g.index]
             for b in range(len(chain), known // P):
                 parent = chain[-1] if chain else 0
@@ -308,6 +311,32 @@ class CacheManager:
                     chain.append(g.pool.register_full_page(table[b], parent, rc.tokens[b * P:(b + 1) * P]))
                 else:               # a window gave the page back before its tokens were known
                     chain.append(hash_block(parent, rc.tokens[b * P:(b + 1) * P]))
+
+    def make_private(self, rc: RequestCache, group: int) -> None:
+        """Take a request's pages of a group out of sharing, before entries are moved within them (``ops.evict_tokens``): nobody who is
+        opened later finds them by their tokens, now or when more of them become full, and pages that others hold too are
+        replaced by copies of its own.  Copies that are asked for (here or by requests opened before) are to be made before anything is
+        moved: ``page_copies_by_group`` and ``ops.copy_pages``, as at the beginning of a step.  All or nothing: on OutOfPages
+        everything is as it was."""
+        if rc.closed:
+            raise RuntimeError(f"request {rc.req_id!r} is closed")
+        g = self.groups[group]
+        if not g.is_paged:
+            raise ValueError(f"group {group} has no pages")
+        table = rc.tables[group]
+        shared = [b for b, p in enumerate(table) if p >= 0 and g.pool.refcounts[p] > 1]
+        if len(shared) > g.pool.num_free:
+            raise OutOfPages(f"{len(shared)} pages of request {rc.req_id!r} are shared and {g.pool.num_free} are free")
+        for p in table:
+            if p >= 0 and g.pool.refcounts[p] == 1:
+                g.pool.unregister_page(p)
+        for b in shared:
+            old, new = table[b], g.pool.allocate()
+            table[b] = new
+            self._page_copies.append((group, old, new))
+            g.pool.release(old)
+        rc.private.add(group)
+        self.peak_pages_used = max(self.peak_pages_used, self.pages_in_use())
 
     def resolve_token(self, rc: RequestCache, position: int, token: int) -> None:
         """The id of a token that was run before it was known on the host (a step launched ahead

@@ -105,6 +105,13 @@ class PagePool:
         self._tokens_of_page.pop(page, None)
 
     # ---- sharing ----------------------------------------------------------------------
+    def unregister_page(self, page: int) -> None:
+        """A held page that will no longer hold its tokens' entries in their order: nobody finds it from now on."""
+        self._check_id(page)
+        if self.refcounts[page] <= 0:
+            raise RuntimeError(f"cannot unregister free page {page}")
+        self._forget_hash(page)
+
     def register_full_page(self, page: int, parent_hash: int, tokens: Sequence[int]) -> int:
         """Make a page whose every slot is written findable; returns its hash.
 

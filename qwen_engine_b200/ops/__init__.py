@@ -1900,8 +1900,10 @@ def evict_tokens(cache: torch.Tensor, block_tables: torch.Tensor, slot_ids: torc
     slot_ids int32 [R]: the rows of ``weights`` (float32) and ``positions`` (int32), both [layers, slots, Hkv, capacity], that
     belong to the requests; lens int32 [R] on the device.  weights_out and positions_out get the kept entries' weights and
     positions in their new places (places from min(lens, keep) on stay as they are); they may be the inputs themselves.
-    A request's positions are distinct, pages it moves within are its own (not shared with another request), no two requests
-    have one slot.  ``alloc(shape, dtype)`` gives scratch memory."""
+    A request's positions are distinct, pages it moves within are its own, no two requests have one slot: with a ``CacheManager`` that shares
+    prefixes, ``make_private`` takes a request's pages out of sharing first (also from requests opened later, which would find them by their
+    tokens).  Afterwards the cache holds fewer entries than the request has had tokens: the next step's cached length and its tokens'
+    positions are two numbers, which the caller gives (``RequestCache.num_tokens`` stands for both).  ``alloc(shape, dtype)`` gives scratch memory."""
     _need(cache.dim() == 6 and cache.is_contiguous() and cache.element_size() % 2 == 0,
           "evict_tokens: cache must be contiguous [layers, pages, planes, Hkv, page, D], of two bytes an element or a multiple")
     S, pages, planes, Hkv, page, D = (int(n) for n in cache.shape)

@@ -907,3 +907,39 @@ def test_accumulate_attention_of_prompts_in_wide_tables_asks_for_bounded_scratch
     monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_SCRATCH", 1 << 16)
     _check_weights(c)
     assert sum(asked) <= 6 << 20                  # (the rows' statistics)
+
+
+def test_evict_tokens_from_a_cache_that_was_shared():
+    """A request whose first pages another one holds too: made private (copies as at the beginning of a step) and evicted, it gives what an unshared
+    one gives, the other's pages stay as they are, and a third with the same tokens finds the other's alone."""
+    from qwen_engine_b200.cache import CacheManager, PagedKVSpec
+    Hkv, D, P, n, keep = 2, 64, 16, 150, 40
+    cm = CacheManager([PagedKVSpec(Hkv, D)] * 2, P, 40, 4, torch.bfloat16, DEV)
+    prompt = list(range(200, 200 + n))
+
+    def opened(name, tokens):
+        rc = cm.open(name, tokens, len(tokens))
+        cm.append(rc, tokens[rc.num_tokens:])
+        cm.commit(rc)
+        return rc
+    a, b = opened("a", prompt), opened("b", prompt[:100])
+    assert b.shared_tokens == 96
+    g = torch.Generator().manual_seed(900)
+    cache = cm.groups[0].tensor
+    cache.copy_(torch.randn(cache.shape, generator=g).to(torch.bfloat16))
+    before, table = cache.cpu(), torch.tensor([a.tables[0]], dtype=torch.int32)
+    cm.make_private(a, 0)
+    ops.copy_pages(cache, torch.tensor(cm.page_copies_by_group()[0], dtype=torch.int32, device=DEV))
+    mine = torch.tensor([a.tables[0]], dtype=torch.int32)
+    w, pos = torch.rand(2, 1, Hkv, n, generator=g), torch.arange(n, dtype=torch.int32).expand(2, 1, Hkv, n).contiguous()
+    slot, lens = torch.zeros(1, dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    want = plain_drafts.evict(before, table, slot, lens, w, pos, w, pos, keep, 2, 8)
+    dw, dp = w.to(DEV), pos.to(DEV)
+    ops.evict_tokens(cache, mine.to(DEV), slot.to(DEV), lens.to(DEV), dw, dp, dw, dp, keep, 2, 8, _alloc)
+    after = cache.cpu()
+    assert torch.equal(after[:, mine[0].long()], want[0][:, table[0].long()]) and torch.equal(dw.cpu(), want[1]) and torch.equal(dp.cpu(), want[2])
+    theirs = torch.tensor(b.tables[0])
+    assert torch.equal(after[:, theirs], before[:, theirs])
+    c = cm.open("c", prompt, n)
+    assert c.shared_tokens == 96 and c.tables[0] == b.tables[0][:6]
+    cm.check_invariants()

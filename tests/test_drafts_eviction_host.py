@@ -166,3 +166,69 @@ def test_kernels_are_configured_for_every_device_they_run_on():
         assert "static bool" not in source, name
         for at in re.finditer("cudaFuncSetAttribute", source):
             assert "qe_once_a_device(" in source[max(0, at.start() - 120):at.start()], name
+
+
+def _manager(num_pages=12):
+    from qwen_engine_b200.cache import CacheManager, PagedKVSpec
+    return CacheManager([PagedKVSpec(2, 8)] * 2 + [PagedKVSpec(1, 8)], 4, num_pages, 6, torch.float32, "cpu")
+
+
+def _opened(cm, name, tokens):
+    rc = cm.open(name, tokens, len(tokens))
+    cm.append(rc, tokens[rc.num_tokens:])
+    cm.commit(rc)
+    return rc
+
+
+def test_private_pages_are_not_found_by_their_tokens():
+    """Pages within which entries are moved: a request that is opened later with the same tokens must not get them, neither those that were full
+    when they became private nor those that become full afterwards."""
+    prompt = list(range(30, 42))
+    cm = _manager()
+    a = _opened(cm, "a", prompt[:10])
+    cm.make_private(a, 0)
+    assert cm.open("b", prompt, 12).shared_tokens == 0
+    cm.close(cm.live["b"])
+    cm.append(a, prompt[10:])
+    cm.commit(a)
+    assert cm.open("c", prompt, 12).shared_tokens == 0 and cm.page_copies_by_group() == {}
+    cm.check_invariants()
+    # ... nor when they have been given back
+    cm.close(a)
+    cm.close(cm.live["c"])
+    assert cm.open("d", prompt, 12).shared_tokens == 0
+    cm.check_invariants()
+
+
+def test_pages_that_others_hold_are_copied_before_they_become_private():
+    prompt = list(range(30, 42))
+    cm = _manager()
+    a = _opened(cm, "a", prompt)
+    b = _opened(cm, "b", prompt[:9])
+    assert b.shared_tokens == 8
+    held = list(b.tables[0])
+    cm.make_private(a, 0)
+    assert b.tables[0] == held and a.tables[0][:2] != held[:2] and not set(a.tables[0]) & set(held)
+    assert cm.page_copies_by_group() == {0: [held[0], a.tables[0][0], held[1], a.tables[0][1]]}
+    assert a.tables[1][:2] == b.tables[1][:2]             # (the other group's are as they were)
+    cm.check_invariants()
+    # b's stay findable; a's third page was found through no copy
+    c = cm.open("c", prompt, 12)
+    assert c.shared_tokens == 8 and c.tables[0] == held[:2]
+    cm.check_invariants()
+    for rc in (a, b, c):
+        cm.close(rc)
+    cm.check_invariants()
+
+
+def test_pages_do_not_become_private_by_halves():
+    from qwen_engine_b200.cache import OutOfPages
+    prompt = list(range(30, 42))
+    cm = _manager(num_pages=5)
+    a, b = _opened(cm, "a", prompt), _opened(cm, "b", prompt[:9])
+    tables = [list(a.tables[0]), list(b.tables[0])]
+    with pytest.raises(OutOfPages):
+        cm.make_private(a, 0)
+    assert [a.tables[0], b.tables[0]] == tables and cm.page_copies_by_group() == {} and not a.private
+    assert cm.open("c", prompt, 12).shared_tokens == 11   # (all of it is found; the last page is copied)
+    cm.check_invariants()
