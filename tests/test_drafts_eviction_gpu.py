@@ -943,3 +943,15 @@ def test_evict_tokens_from_a_cache_that_was_shared():
     c = cm.open("c", prompt, n)
     assert c.shared_tokens == 96 and c.tables[0] == b.tables[0][:6]
     cm.check_invariants()
+
+
+@pytest.mark.parametrize("dtype,q_lens,tc,want", [(torch.bfloat16, [33, 200], True, {"qe_attention_weights_tc"}), (torch.bfloat16, [33, 200], False, {"qe_attention_weights"}),
+                                                  (torch.bfloat16, [1, 8], True, {"qe_attention_weights_few"}), (torch.float32, [1, 200], True, {"qe_attention_weights"}),
+                                                  (torch.bfloat16, [1, 200], True, {"qe_attention_weights_few", "qe_attention_weights_tc"}),
+                                                  (torch.bfloat16, [1, 200], False, {"qe_attention_weights_few", "qe_attention_weights"})])
+def test_which_kernels_gather_attention_weights(dtype, q_lens, tc, want, monkeypatch):
+    called, entry = set(), ops._entry
+    monkeypatch.setattr(ops, "_entry", lambda name: called.add(name) or entry(name))
+    monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_TC", tc)
+    _check_weights(_weights_case(dtype, 8, 2, 128, 16, q_lens, [40, 7], 92))
+    assert called == want

@@ -232,3 +232,12 @@ def test_pages_do_not_become_private_by_halves():
     assert [a.tables[0], b.tables[0]] == tables and cm.page_copies_by_group() == {} and not a.private
     assert cm.open("c", prompt, 12).shared_tokens == 11   # (all of it is found; the last page is copied)
     cm.check_invariants()
+
+
+def test_parts_of_prompts_give_every_sm_a_unit():
+    """As many parts as give every SM one, and no more; four tiles of the other side a part at least."""
+    for units in (1, 2, 7, 64, 74, 147, 148, 149, 1000):
+        for tiles in (1, 3, 4, 5, 100, 1000):
+            parts = ops.attention_weights_tc_parts(units, tiles)
+            assert 1 <= parts <= min(max(1, -(-tiles // 4)), ops.ATTENTION_WEIGHTS_MAX_PARTS) and (parts == 1 or (parts - 1) * units < 148)
+            assert parts * units >= 148 or parts in (-(-tiles // 4), ops.ATTENTION_WEIGHTS_MAX_PARTS)
