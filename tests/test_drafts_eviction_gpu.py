@@ -955,3 +955,25 @@ def test_which_kernels_gather_attention_weights(dtype, q_lens, tc, want, monkeyp
     monkeypatch.setattr(ops, "ATTENTION_WEIGHTS_TC", tc)
     _check_weights(_weights_case(dtype, 8, 2, 128, 16, q_lens, [40, 7], 92))
     assert called == want
+
+
+@pytest.mark.parametrize("V", [7, 1001, 32003, 151935])
+def test_verify_drafts_that_fall_where_both_distributions_are_one(V):
+    """Drafts that can only fall (outside the vocabulary, or masked in both models) where the draft model's logits are the target's, rows on every boundary:
+    nothing is left of max(p - q, 0), not a rounding either, and the token comes from p."""
+    for seed, top_ks in ((0, (0,)), (1, (0, 5))):
+        c = _verify_case(6, [1, 3], V, 950 + seed, True, top_ks=top_ks, temps=(0.7, 1.0, 1.3))
+        starts = c["row_starts"].tolist()
+        rows = [starts[r] + i for r in range(6) for i in range(starts[r + 1] - starts[r] - 1)]
+        for j, row in enumerate(rows):
+            if j % 2:
+                c["draft_tokens"][j] = V
+            else:
+                c["draft_tokens"][j] = j % V
+                c["logits"][row, j % V] = -math.inf
+        c["draft_logits"] = c["logits"][rows].clone()
+        want = plain_drafts.verify(**c)
+        assert (want[1] == 1).all()
+        for u in (0.05, 0.3, 0.5, 0.8, 0.99):
+            c["uniform"][:] = u
+            _same(_verify(c), plain_drafts.verify(**c))
