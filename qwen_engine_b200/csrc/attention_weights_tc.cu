@@ -11,11 +11,13 @@
 //
 // A unit is a (request, kv head, group of A tiles) and a part of the B tiles; parts are merged by a small kernel behind each
 // pass, in their order, so sums do not depend on which CTA was first.  Between the passes it leaves -log2 of every row's whole
-// sum, exponentials and maximum together, in the order of the second pass's columns: a weight is then one exponential.
+// sum, exponentials and maximum together, in the order of the second pass's columns: a weight is then one exponential.  That number is rounded
+// to float32, so a weight is off by up to 2^-24 ln 2 times its size relative to itself, as it is by the rounding of its score.
 //
 // What bounds it: a product of 128 x 128 x 128 takes the tensor cores 512 cycles at best (both operands from shared memory, 8 KB every 64 cycles, are
-// all that it delivers; measured, with the readers beside it, about 950), its 16 384 exponentials the special-function unit 1 024, and the
-// readers' instructions their issue slots about as long.  An eighth of the exponentials is a polynomial (at2_poly2), two at a time on the float32
+// all that it delivers; measured, with the readers beside it, about 950), its 16 384 exponentials the special-function unit 1 024.  No unit is
+// saturated (4 096 tokens: special functions 65 % of an SM's cycles, tensor cores 36 and 40 %, issue slots 45 and 41 %; the passes 105 and 131 us on
+// cold caches): a group of readers has one accumulator, which the next product gets when its last columns have been read, and waits for it.  An eighth of the exponentials is a polynomial (at2_poly2), two at a time on the float32
 // units: none 256, an eighth 249, a quarter 259, three eighths 271 us for a prompt of 4 096 tokens with 32 / 8 heads (one CTA walking several
 // units 269: some are empty, and they are dealt out beforehand; 128 x 256 products in two accumulators 258).  With all heads' longest units first and
 // a unit an SM instead of four: 217.

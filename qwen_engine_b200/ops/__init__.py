@@ -1790,7 +1790,8 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
     ``counted`` (int32 [R]): only so many of a request's first rows count (what ``verify_drafts`` leaves in its counts);
     the others' keys get no weight.
     ``window``, ``slopes``, ``softcap``, ``sinks``: as in ``paged_attention``.  Keys that lie in no page get no weight; distances
-    are of places in the cache, so that a window or a distance bias goes with a cache that nothing was evicted from.
+    are of places in the cache, so that a window or a distance bias goes with a cache that nothing was evicted from.  A row that sees a NaN (in its
+    query or in a key) makes NaN of every key it sees.
     ``alloc(shape, dtype)`` gives scratch memory, ATTENTION_WEIGHTS_SCRATCH bytes of it for scores or sums (more, up to ATTENTION_WEIGHTS_SCRATCH_MOST, where the
     lengths that ctx.ctx_lens_host holds need it).  Float32 sums in one order: equal calls give equal bits.  Launches go by the
     requests' tokens (ctx.q_lens_host): a captured call may be replayed with other cached lengths, pages, slots and ``counted``
