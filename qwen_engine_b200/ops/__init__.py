@@ -1818,9 +1818,12 @@ def accumulate_attention(qkv: torch.Tensor, kv_pages: torch.Tensor, block_tables
     _need(scale > 0.0 and softcap >= 0.0, "accumulate_attention: the scale must be positive, the cap not negative")
     q_lens, ctx_lens = ctx.q_lens_host, ctx.ctx_lens_host
     _need(len(q_lens) == R and len(ctx_lens) == R, "accumulate_attention: the context must have the lengths of every request")
-    for t, n in ((ctx.cu_q, R + 1), (ctx.ctx_lens, R), (ctx.slot_ids, R), (ctx.positions, T)):
+    tokens = sum(q_lens)
+    for t, n in ((ctx.cu_q, R + 1), (ctx.ctx_lens, R), (ctx.slot_ids, R), (ctx.positions, tokens)):
         if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
             raise KernelRefused("accumulate_attention: the context's cu_q [R + 1], ctx_lens [R], slot_ids [R] and positions [T] must be contiguous int32")
+    _need(tokens <= T, "accumulate_attention: qkv must hold a row for every token")
+    T = min(T, ctx.positions.numel())             # (rows behind the tokens', of a buffer that is larger, are not looked at)
     pages, planes, _, page, _ = kv_shape
     slots, _, capacity = shape
     blocks = block_tables.shape[1]

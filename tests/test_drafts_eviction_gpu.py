@@ -977,3 +977,52 @@ def test_verify_drafts_that_fall_where_both_distributions_are_one(V):
         for u in (0.05, 0.3, 0.5, 0.8, 0.99):
             c["uniform"][:] = u
             _same(_verify(c), plain_drafts.verify(**c))
+
+
+def test_replayed_with_longer_contexts_than_scratch_memory_was_asked_for(monkeypatch):
+    """A captured call whose scratch memory goes by the lengths at its capture: replayed with longer ones, it gives what eager calls give."""
+    for name in ("ATTENTION_WEIGHTS_SCRATCH", "ATTENTION_WEIGHTS_SCRATCH_MOST"):
+        monkeypatch.setattr(ops, name, 1 << 16)
+    Hq, Hkv, D, q_lens = 8, 2, 64, [4, 1, 3, 2, 4, 1, 1, 2, 3]
+    cases = [_weights_case(torch.bfloat16, Hq, Hkv, D, 16, q_lens, ctx, 960 + i, extra=0) for i, ctx in enumerate(([20 * r for r in range(9)], [1200 - 130 * r for r in range(9)]))]
+    places = 1600
+    cases = [_widen(dict(c, pages=torch.cat([c["pages"], torch.zeros(600 - c["pages"].shape[0], *c["pages"].shape[1:], dtype=c["pages"].dtype)])), places, 16) for c in cases]
+    want = [_check_weights(c) for c in cases]
+    live = {k: cases[0][k].to(DEV) for k in ("qkv", "pages", "table", "weights", "ctx", "slots", "cu", "step_positions")}
+    out = torch.full_like(live["weights"], -5.0)
+    ctx = SimpleNamespace(num_reqs=9, cu_q=live["cu"], ctx_lens=live["ctx"], slot_ids=live["slots"], positions=live["step_positions"], q_lens_host=q_lens,
+                          ctx_lens_host=cases[0]["ctx_lens"], max_q_len=4)
+
+    def call():
+        ops.accumulate_attention(live["qkv"], live["pages"], live["table"], ctx, live["weights"], out, D ** -0.5, 0, Hq, Hkv, D, _alloc)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        call()
+    for i in (1, 0, 1):
+        for k, x in live.items():
+            x.copy_(cases[i][k])
+        out.fill_(-5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.cpu(), want[i])
+
+
+@pytest.mark.parametrize("dtype,q_lens", [(torch.float32, [3, 40]), (torch.bfloat16, [3, 1]), (torch.bfloat16, [3, 140])])
+def test_accumulate_attention_of_rows_in_a_larger_buffer(dtype, q_lens):
+    """Rows behind the step's tokens (NaN here) are not looked at, with positions for them and without."""
+    c = _weights_case(dtype, 8, 2, 64, 16, q_lens, [50, 9], 970)
+    want = _check_weights(c)
+    c["qkv"] = torch.cat([c["qkv"], torch.full((5, c["qkv"].shape[1]), math.nan, dtype=dtype)])
+    assert torch.equal(_check_weights_of_tokens(c, q_lens), want)
+    c["step_positions"] = torch.cat([c["step_positions"], torch.full((5,), -4, dtype=torch.int32)])
+    assert torch.equal(_check_weights_of_tokens(c, q_lens), want)
+
+
+def _check_weights_of_tokens(c, q_lens):
+    got, noted = _gather(c)
+    for r, n in enumerate(q_lens):
+        k, a = c["ctx_lens"][r], int(c["cu"][r])
+        assert (noted[int(c["slots"][r]), :, k:k + n] == c["step_positions"][a:a + n]).all()
+    return got

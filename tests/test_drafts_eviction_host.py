@@ -142,7 +142,7 @@ def test_the_entry_points_take_what_the_fronts_give():
     ("cu_q", torch.tensor([0, 2, 3])), ("cu_q", torch.tensor([0, 2], dtype=torch.int32)), ("cu_q", torch.zeros(6, dtype=torch.int32)[::2]),
     ("ctx_lens", torch.tensor([5, 9])), ("ctx_lens", torch.tensor([5], dtype=torch.int32)), ("slot_ids", torch.tensor([0, 2])),
     ("slot_ids", torch.tensor([0], dtype=torch.int32)), ("positions", torch.zeros(3, dtype=torch.int64)), ("positions", torch.zeros(2, dtype=torch.int32)),
-    ("q_lens_host", [2]), ("ctx_lens_host", [5, 9, 1])])
+    ("q_lens_host", [2]), ("ctx_lens_host", [5, 9, 1]), ("q_lens_host", [2, 2])])
 def test_accumulate_attention_refuses_a_context_that_does_not_fit(name, value):
     """What the kernels read of the step's context: int32, a number for every request (cu_q one more) and for every row."""
     args = _weights_args()
